@@ -16,7 +16,7 @@ OUT = os.path.join(HERE, "src", "ffi.rs")
 
 SCALARS = {"int": "i32", "int32_t": "i32", "uint32_t": "u32", "int8_t": "i8", "uint16_t": "u16", "uint64_t": "u64", "int64_t": "i64", "size_t": "usize",
            "float": "f32", "double": "f64", "char": "std::ffi::c_char", "void": "std::ffi::c_void", "pi_status": "i32", "pi_split": "i32"}
-OPAQUE = ["pi_ctx", "pi_linear", "pi_kv_pool", "pi_model", "pi_state_pool"]
+OPAQUE = ["pi_ctx", "pi_linear", "pi_kv_pool", "pi_model", "pi_state_pool", "pi_kv8_pool"]
 
 
 def rust_name(c: str) -> str:

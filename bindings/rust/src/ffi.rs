@@ -32,6 +32,8 @@ pub const PI_SPLIT_ROW: i32 = 2;
 pub const PI_F32: i32 = 0;
 pub const PI_INT8: i32 = 1;
 pub const PI_BF16: i32 = 2;
+pub const PI_F16: i32 = 3;
+pub const PI_E4M3: i32 = 4;
 pub const PI_MIXER_ATTENTION: i32 = 0;
 pub const PI_MIXER_GLA: i32 = 1;
 pub const PI_MIXER_MLSTM: i32 = 2;
@@ -59,6 +61,7 @@ pub const PI_TP_PEER_HANDLE_BYTES: i32 = 64;
 #[repr(C)] pub struct PiKvPool { _private: [u8; 0] }
 #[repr(C)] pub struct PiModel { _private: [u8; 0] }
 #[repr(C)] pub struct PiStatePool { _private: [u8; 0] }
+#[repr(C)] pub struct PiKv8Pool { _private: [u8; 0] }
 
 #[repr(C)]
 #[derive(Clone, Copy)]
@@ -212,6 +215,22 @@ pub struct PiStepBatch {
     pub out_rows: *const i32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct PiStepArrays {
+    pub block_size: i32,
+    pub max_seqs: i32,
+    pub max_blocks: i32,
+    pub max_rows: i32,
+    pub tables: *mut i32,
+    pub lens: *mut i32,
+    pub cu_rows: *mut i32,
+    pub row_seq: *mut i32,
+    pub row_pos: *mut i32,
+    pub slots: *mut i64,
+    pub counts: *mut i32,
+}
+
 extern "C" {
     pub fn pi_version() -> *const std::ffi::c_char;
     pub fn pi_last_error(ctx: *const PiCtx) -> *const std::ffi::c_char;
@@ -283,4 +302,14 @@ extern "C" {
     pub fn pi_model_step_multi(ctx: *mut PiCtx, model: *mut PiModel, pool: *mut PiKvPool, state_or_null: *mut PiStatePool, batch: *const PiStepBatch, n_steps: i32, out_tokens_host: *mut u32) -> i32;
     pub fn pi_model_trace_layers(ctx: *mut PiCtx, model: *mut PiModel, on: i32) -> i32;
     pub fn pi_model_read_layer(ctx: *mut PiCtx, model: *const PiModel, layer: i32, rows: i32, x_host_out: *mut f32) -> i32;
+    pub fn pi_step_plan(ctx: *mut PiCtx, arrays: *const PiStepArrays, start_dev: *const i32, n_tokens_dev: *const i32, n_seqs: i32, free_dev: *const i32, n_free: i32) -> i32;
+    pub fn pi_kv8_pool_create(ctx: *mut PiCtx, layout: *const PiKvLayout, kind: i32, codes_dev_or_null: *mut std::ffi::c_void, scales_dev_or_null: *mut f32, out: *mut *mut PiKv8Pool) -> i32;
+    pub fn pi_kv8_pool_destroy(pool: *mut PiKv8Pool);
+    pub fn pi_kv8_pool_bytes(pool: *const PiKv8Pool) -> usize;
+    pub fn pi_kv8_pool_pitch(pool: *const PiKv8Pool) -> i32;
+    pub fn pi_kv8_copy_block(ctx: *mut PiCtx, pool: *mut PiKv8Pool, src: i32, dst: i32) -> i32;
+    pub fn pi_kv8_read_token(ctx: *mut PiCtx, pool: *const PiKv8Pool, layer: i32, block: i32, tok: i32, k_host_out: *mut f32, v_host_out: *mut f32) -> i32;
+    pub fn pi_kv8_write(ctx: *mut PiCtx, pool: *mut PiKv8Pool, layer: i32, dtype: i32, k_dev: *const std::ffi::c_void, k_stride: usize, v_dev: *const std::ffi::c_void, v_stride: usize, slots_dev: *const i64, n_rows: i32) -> i32;
+    pub fn pi_kv8_attention(ctx: *mut PiCtx, pool: *const PiKv8Pool, layer: i32, num_heads: i32, dtype: i32, q_dev: *const std::ffi::c_void, q_stride: usize, out_dev: *mut std::ffi::c_void, out_stride: usize, arrays: *const PiStepArrays, n_seqs: i32, n_rows: i32, max_seq_rows: i32, max_context: i32, window: i32, scale: f32) -> i32;
+    pub fn pi_sample(ctx: *mut PiCtx, logits_dev: *const std::ffi::c_void, dtype: i32, row_stride: usize, rows: i32, n: i32, temperature_dev: *const f32, top_k_dev: *const i32, top_p_dev: *const f32, min_p_dev: *const f32, u_dev: *const f32, ids_dev: *mut i32, probs_dev_or_null: *mut f32) -> i32;
 }

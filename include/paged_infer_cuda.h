@@ -24,7 +24,7 @@
  *    calls that only touch device memory are ordered on the context's stream.
  *  - Matrices are row-major [out_features][in_features] (y = x * W^T), as in the
  *    reference (src/model.rs:140-199).
- *  - The device layout of weights and of the KV pool is private to the library.
+ *  - The device layout of weights and of the KV pool is private to the library (that of the 8-bit pool is documented).
  */
 #ifndef PAGED_INFER_CUDA_H
 #define PAGED_INFER_CUDA_H
@@ -52,6 +52,7 @@ typedef struct pi_linear pi_linear;
 typedef struct pi_kv_pool pi_kv_pool;
 typedef struct pi_model pi_model;
 typedef struct pi_state_pool pi_state_pool;
+typedef struct pi_kv8_pool pi_kv8_pool;
 
 /* ---- context --------------------------------------------------------------- */
 
@@ -140,7 +141,7 @@ pi_status pi_quantize_rows_i8_dev(pi_ctx* ctx, const float* w_dev, size_t rows, 
 /* ---- projections ------------------------------------------------------------- */
 
 typedef enum { PI_SPLIT_NONE = 0, PI_SPLIT_COLUMN = 1, PI_SPLIT_ROW = 2 } pi_split;
-enum { PI_F32 = 0, PI_INT8 = 1, PI_BF16 = 2 };
+enum { PI_F32 = 0, PI_INT8 = 1, PI_BF16 = 2, PI_F16 = 3, PI_E4M3 = 4 /* 8-bit floating point, 4 bits of exponent */ };
 
 /* Replaces: QuantizedLinear {rows, cols, weight, scales} (src/model.rs:164-199).
  * The codes and scales are copied to the device (sharded per `split` on a
@@ -501,6 +502,92 @@ pi_status pi_model_step_multi(pi_ctx* ctx, pi_model* model, pi_kv_pool* pool, pi
  * numerical tests: ask for it with pi_model_trace_layers(model, 1) before the step. */
 pi_status pi_model_trace_layers(pi_ctx* ctx, pi_model* model, int on);
 pi_status pi_model_read_layer(pi_ctx* ctx, const pi_model* model, int layer, int rows, float* x_host_out);
+
+/* ---- the device side of a serving step over an 8-bit KV cache --------------------------------------------------
+ * A step of a ragged batch without a round trip to the host: its block tables and slots are made on the device from the
+ * lengths of its requests, its keys and values are stored as 8-bit codes, attention reads those, and its tokens are drawn
+ * from logits on the device.  All pointers are device memory on the context's device, all calls are ordered on the
+ * context's stream, allocate nothing, wait for nothing on the host and may be captured into a CUDA graph (after a first
+ * call of the same kind outside one); none of them keeps scratch memory, so contexts and graphs never share any.
+ * No counterpart in the reference. */
+
+/* The arrays of a step, all the caller's.  Rows are numbered through, sequence by sequence. */
+typedef struct {
+  int32_t block_size;      /* tokens of a block */
+  int32_t max_seqs;        /* sequences that tables, lens and cu_rows have room for */
+  int32_t max_blocks;      /* entries of a row of the tables */
+  int32_t max_rows;        /* rows that row_seq, row_pos and slots have room for */
+  int32_t* tables;         /* [max_seqs][max_blocks] physical block ids, -1: none */
+  int32_t* lens;           /* [max_seqs] entries of a row that are in use */
+  int32_t* cu_rows;        /* [max_seqs + 1] first row of each sequence */
+  int32_t* row_seq;        /* [max_rows] sequence of a row, -1 behind the last */
+  int32_t* row_pos;        /* [max_rows] position of a row in its sequence, -1 behind the last */
+  int64_t* slots;          /* [max_rows] block id * block_size + place in the block; -1: behind the last row, or not mapped */
+  int32_t* counts;         /* [3] rows that the lengths ask for, blocks taken, blocks that were not to be had */
+} pi_step_arrays;
+
+/* Sequence b holds start[b] tokens and brings n_tokens[b] >= 0 more (a negative number counts as 0).  The first
+ * ceil(start / block_size) entries of its table are the caller's and stay; the entries up to
+ * ceil((start + n_tokens) / block_size) are written from the free list, sequence by sequence, from its front on.  lens,
+ * cu_rows, row_seq, row_pos, slots and counts are written for the n_seqs sequences and all max_rows rows; entries of a
+ * table behind its length and tables behind the last sequence stay as they are.  The call changes none of its inputs:
+ * the caller drops the first counts[1] ids from the free list.  Where the list runs out, or a row of the tables is full,
+ * entries become -1 (or do not exist), slots become -1 and counts[2] says how many blocks were missing; rows beyond
+ * max_rows are left out (counts[0] still counts them).  At most 16384 sequences; positions stay below 2^31. */
+pi_status pi_step_plan(pi_ctx* ctx, const pi_step_arrays* arrays, const int32_t* start_dev, const int32_t* n_tokens_dev, int n_seqs,
+                       const int32_t* free_dev, int n_free);
+
+/* A pool of 8-bit codes: codes [layer][block][kv_head][k|v][token][pitch] of kind PI_INT8 or PI_E4M3, scales
+ * [layer][block][kv_head][k|v] f32, value = code * scale.  pitch is head_dim rounded up to 32, 64, 96, 128, 192 or 256
+ * bytes; the bytes behind head_dim are written as zeros.  codes_dev (16-byte aligned) and scales_dev (8-byte aligned) are
+ * memory of the caller in this layout that outlives the pool, or both NULL: the pool allocates its own, contents undefined.
+ * head_dim <= 256, block_size <= 4096, num_kv_heads <= 1024. */
+pi_status pi_kv8_pool_create(pi_ctx* ctx, const pi_kv_layout* layout, int kind, void* codes_dev_or_null, float* scales_dev_or_null,
+                             pi_kv8_pool** out);
+void pi_kv8_pool_destroy(pi_kv8_pool* pool);
+size_t pi_kv8_pool_bytes(const pi_kv8_pool* pool);
+int pi_kv8_pool_pitch(const pi_kv8_pool* pool);
+/* Duplicate one physical block, codes and scales, across all layers (copy-on-write).  src == dst is PI_ERR_INVALID_ARG. */
+pi_status pi_kv8_copy_block(pi_ctx* ctx, pi_kv8_pool* pool, int32_t src, int32_t dst);
+/* One token's K and V ([num_kv_heads x head_dim] each) of one layer, as the values that the codes stand for. */
+pi_status pi_kv8_read_token(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int32_t block, int tok, float* k_host_out,
+                            float* v_host_out);
+
+/* Store the keys and values of n_rows rows of one layer at slots[row]; a row with a slot below 0 or outside the pool is
+ * skipped.  k_dev and v_dev: [n_rows][num_kv_heads][head_dim] of kind PI_F32, PI_BF16 or PI_F16, k_stride and v_stride
+ * values from row to row.  Neighbouring rows of one block are stored together; the rows of a block must be neighbours, in
+ * the order of their slots, and start at the block's first token or behind the tokens already stored.  Per head and side
+ * (K or V) the block's scale becomes the larger of its scale so far (none, where the rows start at the block's first token)
+ * and the rows' largest magnitude times 1/127 (PI_INT8) or 1/448 (PI_E4M3) as an f32; codes are value / scale, rounded to nearest, halves
+ * away from zero (PI_INT8) or to even (PI_E4M3); where the scale grows, the codes in front are encoded again.  Tokens
+ * behind the stored ones become void.  A value that is not finite makes the scale NaN until the block is written from its
+ * first token on again. */
+pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, const void* k_dev, size_t k_stride, const void* v_dev,
+                       size_t v_stride, const int64_t* slots_dev, int n_rows);
+
+/* Row r of sequence b (cu_rows[b] <= r < cu_rows[b + 1]) attends positions max(0, p - window + 1) ..= p, p = row_pos[r],
+ * of its sequence (window <= 0: from 0 on); positions in blocks that are not mapped (behind lens[b], id below 0 or outside
+ * the pool) are left out, and a row that sees nothing yields zeros.  q and out: [n_rows][num_heads][head_dim] of kind
+ * PI_F32, PI_BF16 or PI_F16, q_stride and out_stride values from row to row; query head h reads KV head
+ * h / (num_heads / num_kv_heads).  Weights are softmax(scale q k), accumulated in f32.  tables, lens, cu_rows and row_pos
+ * of `arrays` are read (the others may be NULL), of its first n_seqs sequences; rows outside every sequence are not written.
+ * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut;
+ * results do not depend on their being right. */
+pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int num_heads, int dtype, const void* q_dev, size_t q_stride,
+                           void* out_dev, size_t out_stride, const pi_step_arrays* arrays, int n_seqs, int n_rows, int max_seq_rows,
+                           int max_context, int window, float scale);
+
+/* Draw a token from each of `rows` rows of n logits (PI_F32, PI_BF16 or PI_F16, row_stride values from row to row), with
+ * parameters per row, all on the device.  With weights w = exp((logit - largest) / temperature) and tokens ordered by
+ * logit, equal ones by index: kept are the first top_k (top_k <= 0 or >= n: all), of those the ones with w >= min_p
+ * (min_p <= 0: all), of those the shortest beginning whose weights reach top_p of the sum (top_p >= 1: all; at least one
+ * token).  ids gets the first kept token, in the order of indices, whose running sum of weights exceeds u times their
+ * sum; u is in [0, 1).  probs (may be NULL) gets its weight over that sum.  temperature <= 0: the largest logit, the
+ * lowest index of equal ones, with probability 1.  A NaN logit counts as minus infinity; a row of nothing else gives
+ * id -1 and probability 0.  Results do not depend on how the work is divided.  n <= 393216. */
+pi_status pi_sample(pi_ctx* ctx, const void* logits_dev, int dtype, size_t row_stride, int rows, int n, const float* temperature_dev,
+                    const int32_t* top_k_dev, const float* top_p_dev, const float* min_p_dev, const float* u_dev, int32_t* ids_dev,
+                    float* probs_dev_or_null);
 
 #ifdef __cplusplus
 }

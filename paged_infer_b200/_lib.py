@@ -21,7 +21,7 @@ PI_ERR_TIMEOUT = -5
 PI_ERR_UNSUPPORTED = -6
 
 PI_SPLIT_NONE, PI_SPLIT_COLUMN, PI_SPLIT_ROW = 0, 1, 2
-PI_F32, PI_INT8, PI_BF16 = 0, 1, 2
+PI_F32, PI_INT8, PI_BF16, PI_F16, PI_E4M3 = 0, 1, 2, 3, 4
 PROF_CLASSES = ("gemv", "gemm_tc", "attention", "rope_kv", "other", "collective", "recurrence")
 PI_OPT_TENSOR_GEMM, PI_OPT_CUDA_GRAPH, PI_OPT_PDL, PI_OPT_GEMV_MAX_M, PI_OPT_ATTN_TMA, PI_OPT_FUSE_PLANES, PI_OPT_ATTN_SHARED = 1, 2, 3, 4, 5, 6, 7
 PI_OPT_PEER_SPIN_LIMIT = 8
@@ -87,6 +87,11 @@ class NamedTensorC(C.Structure):
 class StepBatchC(C.Structure):
     _fields_ = [("n_seqs", C.c_int32), ("tokens", C.c_void_p), ("n_tokens", C.c_void_p), ("start_pos", C.c_void_p), ("block_tables", C.c_void_p),
                 ("max_blocks", C.c_int32), ("table_lens", C.c_void_p), ("state_slots", C.c_void_p), ("n_out", C.c_int32), ("out_rows", C.c_void_p)]
+
+
+class StepArraysC(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("block_size", "max_seqs", "max_blocks", "max_rows")] + \
+               [(n, C.c_void_p) for n in ("tables", "lens", "cu_rows", "row_seq", "row_pos", "slots", "counts")]
 
 
 _P = C.c_void_p
@@ -166,6 +171,16 @@ SIGNATURES = {
     "pi_model_step_multi": (_I, [_P, _P, _P, _P, C.POINTER(StepBatchC), _I, _P]),
     "pi_model_trace_layers": (_I, [_P, _P, _I]),
     "pi_model_read_layer": (_I, [_P, _P, _I, _I, _P]),
+    "pi_step_plan": (_I, [_P, _P, _P, _P, _I, _P, _I]),
+    "pi_kv8_pool_create": (_I, [_P, C.POINTER(KvLayoutC), _I, _P, _P, _PP]),
+    "pi_kv8_pool_destroy": (None, [_P]),
+    "pi_kv8_pool_bytes": (_SZ, [_P]),
+    "pi_kv8_pool_pitch": (_I, [_P]),
+    "pi_kv8_copy_block": (_I, [_P, _P, C.c_int32, C.c_int32]),
+    "pi_kv8_read_token": (_I, [_P, _P, _I, C.c_int32, _I, _P, _P]),
+    "pi_kv8_write": (_I, [_P, _P, _I, _I, _P, _SZ, _P, _SZ, _P, _I]),
+    "pi_kv8_attention": (_I, [_P, _P, _I, _I, _I, _P, _SZ, _P, _SZ, _P, _I, _I, _I, _I, _I, C.c_float]),
+    "pi_sample": (_I, [_P, _P, _I, _SZ, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lib = None

@@ -15,7 +15,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import PI_BF16, PI_F32, PI_INT8, PI_SPLIT_COLUMN, PI_SPLIT_NONE, PI_SPLIT_ROW, PiError, check
+from ._lib import PI_BF16, PI_E4M3, PI_F16, PI_F32, PI_INT8, PI_SPLIT_COLUMN, PI_SPLIT_NONE, PI_SPLIT_ROW, PiError, check
 from .loader import QUANT_F32, QUANT_INT8, HostWeights, LayeredConfig, LlamaConfig
 
 
@@ -503,6 +503,194 @@ class PagedAttention:
                                                  _ptr(mat), mb if mb else 0, _ptr(lens), _ptr(pos), _ptr(start), B),
               kv_cache.ctx.handle)
         return out
+
+
+# ---- the device side of a step over an 8-bit cache ---------------------------------------------------------------------
+
+_KINDS = {"torch.float32": PI_F32, "torch.bfloat16": PI_BF16, "torch.float16": PI_F16}
+_CODES = {"torch.int8": PI_INT8, "torch.float8_e4m3fn": PI_E4M3}
+
+
+def _invalid(message: str):
+    raise PiError(_lib.PI_ERR_INVALID_ARG, message)
+
+
+def _on_device(ctx: Context, t, what: str, dtype: str, n: int | None = None, at_least: int = 0) -> int:
+    """Address of a dense tensor of ``dtype`` on the context's device, with ``n`` (or ``at_least`` so many) elements."""
+    if str(t.dtype) != dtype or not t.is_contiguous() or t.get_device() != ctx.device:
+        _invalid(f"{what} must be a dense {dtype} tensor on CUDA device {ctx.device}")
+    if (n is not None and t.numel() != n) or t.numel() < at_least:
+        _invalid(f"{what} has {t.numel()} elements, {n if n is not None else at_least} are needed")
+    return t.data_ptr()
+
+
+def _rows_of(ctx: Context, t, what: str, heads: int, dim: int):
+    """(kind, address, row stride) of [rows, heads, dim] floating-point rows, each of them dense, on the context's device."""
+    kind = _KINDS.get(str(t.dtype))
+    shape = t.shape
+    if kind is None or len(shape) != 3 or shape[1] != heads or shape[2] != dim or t.get_device() != ctx.device:
+        _invalid(f"{what} must be a float32, bfloat16 or float16 tensor [rows, {heads}, {dim}] on CUDA device {ctx.device}")
+    row, head, one = t.stride()
+    if (one != 1 and dim > 1) or (head != dim and heads > 1):
+        _invalid(f"the rows of {what} must be dense")
+    return kind, t.data_ptr(), row
+
+
+class StepPlan:
+    """The device arrays of a ragged step (``pi_step_arrays``): torch CUDA tensors of the caller.
+
+    tables [max_seqs, max_blocks], lens [max_seqs], cu_rows [max_seqs + 1], row_seq and row_pos [max_rows], counts [3] are
+    int32, slots [max_rows] int64.  :meth:`build` fills them on the device from the lengths of the step's requests; a caller
+    that makes them itself leaves out what nobody reads (a write reads slots, attention tables, lens, cu_rows and row_pos).
+    """
+
+    def __init__(self, ctx: Context, block_size: int, tables, lens=None, cu_rows=None, row_seq=None, row_pos=None, slots=None, counts=None):
+        if len(tables.shape) != 2:
+            _invalid("tables must be [sequences, blocks]")
+        seqs, wide = tables.shape
+        self.ctx, self.block_size, self.max_seqs, self.n_seqs = ctx, block_size, seqs, seqs   # n_seqs: of the step at hand
+        self.tables, self.lens, self.cu_rows, self.row_seq, self.row_pos, self.slots, self.counts = tables, lens, cu_rows, row_seq, row_pos, slots, counts
+        rows = [t.numel() for t in (row_seq, row_pos, slots) if t is not None]
+        self.max_rows = min(rows) if rows else 0
+        c = self._c = _lib.StepArraysC(block_size, seqs, wide, self.max_rows)
+        c.tables = _on_device(ctx, tables, "tables", "torch.int32")
+        for name, least in (("lens", seqs), ("cu_rows", seqs + 1), ("row_seq", 0), ("row_pos", 0), ("counts", 3)):
+            t = getattr(self, name)
+            if t is not None:
+                setattr(c, name, _on_device(ctx, t, name, "torch.int32", at_least=least))
+        if slots is not None:
+            c.slots = _on_device(ctx, slots, "slots", "torch.int64")
+        self._ref = C.byref(c)
+
+    def build(self, start_pos, n_tokens, free_blocks) -> None:
+        """``pi_step_plan``: sequence b holds start_pos[b] tokens and brings n_tokens[b]; missing blocks come from the front of
+        free_blocks (all int32 CUDA tensors).  The tables' leading entries, those of the tokens held, are the caller's; the list
+        is not changed: counts[1] says how many of its ids are now in use.  Asynchronous on the context's stream."""
+        n = start_pos.numel()
+        if not (n <= self.max_seqs and n >= 1):
+            _invalid(f"{n} sequences: the arrays have room for {self.max_seqs}")
+        ctx = self.ctx
+        check(_lib.lib().pi_step_plan(ctx.handle, self._ref, _on_device(ctx, start_pos, "start_pos", "torch.int32"),
+                                      _on_device(ctx, n_tokens, "n_tokens", "torch.int32", n), n,
+                                      _on_device(ctx, free_blocks, "free_blocks", "torch.int32"), free_blocks.numel()), ctx.handle)
+        self.n_seqs = n
+
+
+class KvCache8:
+    """A paged KV pool of 8-bit codes with a scale per block of tokens, head and side (``pi_kv8_pool``).
+
+    ``codes`` [layers, blocks, kv_heads, 2, block_size, pitch] (int8, or float8_e4m3fn) and ``scales`` [layers, blocks,
+    kv_heads, 2] (float32) are torch CUDA tensors of the caller, which the cache holds on to; without them the pool allocates
+    its own memory of ``kind`` ``PI_INT8`` or ``PI_E4M3``, contents undefined.  A value is code * scale; :meth:`pitch_of`
+    gives the bytes of a token's codes.
+    """
+
+    def __init__(self, ctx: Context, layout: KvLayout, kind: int | None = None, codes=None, scales=None):
+        self.ctx, self.layout, self.codes, self.scales = ctx, layout, codes, scales
+        at = [None, None]
+        if (codes is None) != (scales is None):
+            _invalid("codes and scales are either both the caller's or both the pool's")
+        if codes is not None:
+            found = _CODES.get(str(codes.dtype))
+            if found is None or kind not in (None, found):
+                _invalid(f"codes of type {codes.dtype}: torch.int8 or torch.float8_e4m3fn, as the kind says, are wanted")
+            kind = found
+            shape = (layout.num_layers, layout.num_blocks, layout.num_kv_heads, 2, layout.block_size, self.pitch_of(layout.head_dim))
+            if tuple(codes.shape) != shape or tuple(scales.shape) != shape[:4]:
+                _invalid(f"codes must be {list(shape)} and scales {list(shape[:4])}")
+            at = [_on_device(ctx, codes, "codes", str(codes.dtype)), _on_device(ctx, scales, "scales", "torch.float32")]
+        self.kind = PI_INT8 if kind is None else kind
+        h = C.c_void_p()
+        c = layout.as_c()
+        check(_lib.lib().pi_kv8_pool_create(ctx.handle, C.byref(c), self.kind, at[0], at[1], C.byref(h)), ctx.handle)
+        self.handle = h
+
+    def close(self):
+        if getattr(self, "handle", None) and _lib is not None:   # module globals are gone at interpreter exit
+            _lib.lib().pi_kv8_pool_destroy(self.handle)
+            self.handle = None
+
+    __del__ = close
+
+    @staticmethod
+    def pitch_of(head_dim: int) -> int:
+        for p in (32, 64, 96, 128, 192, 256):
+            if p >= head_dim:
+                return p
+        _invalid(f"an 8-bit cache takes head_dim <= 256, not {head_dim}")
+
+    def bytes(self) -> int:
+        return int(_lib.lib().pi_kv8_pool_bytes(self.handle))
+
+    def copy_block(self, src: int, dst: int):
+        check(_lib.lib().pi_kv8_copy_block(self.ctx.handle, self.handle, src, dst), self.ctx.handle)
+
+    def read_token(self, layer: int, block: int, tok: int):
+        """K and V of one token as the values that the codes stand for."""
+        n = self.layout.num_kv_heads * self.layout.head_dim
+        k, v = np.empty(n, np.float32), np.empty(n, np.float32)
+        check(_lib.lib().pi_kv8_read_token(self.ctx.handle, self.handle, layer, block, tok, _ptr(k), _ptr(v)), self.ctx.handle)
+        return k, v
+
+    def write(self, plan: StepPlan, k, v, layer: int = 0) -> None:
+        """``pi_kv8_write``: rows k, v [rows, kv_heads, head_dim] (float32, bfloat16 or float16) to ``plan.slots[:rows]``, rows on
+        negative slots skipped.  Asynchronous on the context's stream."""
+        L, ctx = self.layout, self.ctx
+        kind, k_at, k_row = _rows_of(ctx, k, "k", L.num_kv_heads, L.head_dim)
+        kind_v, v_at, v_row = _rows_of(ctx, v, "v", L.num_kv_heads, L.head_dim)
+        rows = k.shape[0]
+        if kind != kind_v or rows != v.shape[0]:
+            _invalid("k and v must have the same type and number of rows")
+        if plan.slots is None or rows > plan.slots.numel() or plan.block_size != L.block_size or plan.ctx.device != ctx.device:
+            _invalid(f"{rows} rows need as many slots, in blocks of {L.block_size} tokens, on CUDA device {ctx.device}")
+        check(_lib.lib().pi_kv8_write(ctx.handle, self.handle, layer, kind, k_at, k_row, v_at, v_row, plan._c.slots, rows), ctx.handle)
+
+
+class PagedAttention8:
+    """Attention over a :class:`KvCache8` for the rows of a ragged step (``pi_kv8_attention``): decoded tokens, portions of
+    prompts, or both."""
+
+    def __init__(self, layout: KvLayout, num_heads: int):
+        self.layout, self.num_heads = layout, num_heads
+
+    def run_device(self, q, out, cache: KvCache8, plan: StepPlan, layer: int = 0, window: int | None = None, scale: float | None = None,
+                   max_seq_rows: int | None = None, max_context: int | None = None) -> None:
+        """out[r] = attention of q[r] ([rows, num_heads, head_dim], one type) over the positions that its place in ``plan`` sees: all up
+        to its own, or the last ``window`` of them.  ``scale`` defaults to head_dim ** -0.5.  ``max_seq_rows`` and ``max_context``,
+        the most rows and the longest context of a sequence, choose how the work is cut; they default to all rows and to what the tables
+        hold, and results do not depend on them.  Asynchronous on the context's stream."""
+        L, ctx = cache.layout, cache.ctx
+        if L.head_dim != self.layout.head_dim or L.num_kv_heads != self.layout.num_kv_heads:
+            _invalid("the cache is not of this attention's layout")
+        kind, q_at, q_row = _rows_of(ctx, q, "q", self.num_heads, L.head_dim)
+        kind_out, out_at, out_row = _rows_of(ctx, out, "out", self.num_heads, L.head_dim)
+        rows = q.shape[0]
+        if kind != kind_out or rows != out.shape[0]:
+            _invalid("q and out must have the same type and number of rows")
+        if plan.ctx.device != ctx.device or plan.lens is None or plan.cu_rows is None or plan.row_pos is None:
+            _invalid(f"attention needs the plan's tables, lens, cu_rows and row_pos on CUDA device {ctx.device}")
+        if window is not None and window < 1:
+            _invalid(f"a window of {window} positions")
+        check(_lib.lib().pi_kv8_attention(ctx.handle, cache.handle, layer, self.num_heads, kind, q_at, q_row, out_at, out_row, plan._ref, plan.n_seqs, rows,
+                                          max(rows, 1) if max_seq_rows is None else max_seq_rows,
+                                          plan._c.max_blocks * plan.block_size if max_context is None else max_context, window or 0,
+                                          L.head_dim ** -0.5 if scale is None else scale), ctx.handle)
+
+
+def sample(ctx: Context, logits, temperature, top_k, top_p, min_p, u, ids, probs=None) -> None:
+    """``pi_sample``: ids[r] (int32) drawn from logits[r] (float32, bfloat16 or float16 [rows, vocab], rows dense) under temperature[r], top_p[r],
+    min_p[r] (float32) and top_k[r] (int32), with the random number u[r] in [0, 1) (float32); probs[r] (float32) its probability among the
+    tokens that were kept.  temperature <= 0 takes the largest logit, the lowest index of equal ones (:func:`argmax` takes the
+    highest).  All are torch CUDA tensors; asynchronous on the context's stream."""
+    kind = _KINDS.get(str(logits.dtype))
+    if kind is None or len(logits.shape) != 2 or logits.get_device() != ctx.device or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        _invalid(f"logits must be a float32, bfloat16 or float16 tensor [rows, vocab] with dense rows on CUDA device {ctx.device}")
+    rows, n = logits.shape
+    f, i = "torch.float32", "torch.int32"
+    check(_lib.lib().pi_sample(ctx.handle, logits.data_ptr(), kind, logits.stride(0), rows, n, _on_device(ctx, temperature, "temperature", f, rows),
+                               _on_device(ctx, top_k, "top_k", i, rows), _on_device(ctx, top_p, "top_p", f, rows), _on_device(ctx, min_p, "min_p", f, rows),
+                               _on_device(ctx, u, "u", f, rows), _on_device(ctx, ids, "ids", i, rows),
+                               None if probs is None else _on_device(ctx, probs, "probs", f, rows)), ctx.handle)
 
 
 # ---- ragged steps, for every model ------------------------------------------------------------------

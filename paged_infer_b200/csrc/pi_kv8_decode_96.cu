@@ -1,0 +1,7 @@
+// Decode attention over the 8-bit cache: the instantiations of these pitches.
+#include "pi_kv8_decode.cuh"
+
+namespace pi_kv8 {
+template pi_status launch_decode_pitch<96>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
+template pi_status launch_decode_pitch<128>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
+}  // namespace pi_kv8
