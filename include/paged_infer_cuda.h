@@ -571,8 +571,8 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
  * PI_F32, PI_BF16 or PI_F16, q_stride and out_stride values from row to row; query head h reads KV head
  * h / (num_heads / num_kv_heads).  Weights are softmax(scale q k), accumulated in f32.  tables, lens, cu_rows and row_pos
  * of `arrays` are read (the others may be NULL), of its first n_seqs sequences; rows outside every sequence are not written.
- * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut;
- * results do not depend on their being right. */
+ * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut,
+ * and with that the order of sums; results are right whatever they say. */
 pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int num_heads, int dtype, const void* q_dev, size_t q_stride,
                            void* out_dev, size_t out_stride, const pi_step_arrays* arrays, int n_seqs, int n_rows, int max_seq_rows,
                            int max_context, int window, float scale);
@@ -582,9 +582,10 @@ pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int 
  * logit, equal ones by index: kept are the first top_k (top_k <= 0 or >= n: all), of those the ones with w >= min_p
  * (min_p <= 0: all), of those the shortest beginning whose weights reach top_p of the sum (top_p >= 1: all; at least one
  * token).  ids gets the first kept token, in the order of indices, whose running sum of weights exceeds u times their
- * sum; u is in [0, 1).  probs (may be NULL) gets its weight over that sum.  temperature <= 0: the largest logit, the
- * lowest index of equal ones, with probability 1.  A NaN logit counts as minus infinity; a row of nothing else gives
- * id -1 and probability 0.  Results do not depend on how the work is divided.  n <= 393216. */
+ * sum; u is in [0, 1).  Weights are held as whole multiples of 2^-45 of the largest: a token below half of that is not
+ * drawn.  probs (may be NULL) gets its weight over that sum.  temperature <= 0: the largest logit, the lowest index of
+ * equal ones, with probability 1.  A NaN logit counts as minus infinity; a row of nothing else gives id -1 and
+ * probability 0.  Results do not depend on how the work is divided.  n <= 393216. */
 pi_status pi_sample(pi_ctx* ctx, const void* logits_dev, int dtype, size_t row_stride, int rows, int n, const float* temperature_dev,
                     const int32_t* top_k_dev, const float* top_p_dev, const float* min_p_dev, const float* u_dev, int32_t* ids_dev,
                     float* probs_dev_or_null);

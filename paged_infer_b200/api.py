@@ -657,8 +657,8 @@ class PagedAttention8:
                    max_seq_rows: int | None = None, max_context: int | None = None) -> None:
         """out[r] = attention of q[r] ([rows, num_heads, head_dim], one type) over the positions that its place in ``plan`` sees: all up
         to its own, or the last ``window`` of them.  ``scale`` defaults to head_dim ** -0.5.  ``max_seq_rows`` and ``max_context``,
-        the most rows and the longest context of a sequence, choose how the work is cut; they default to all rows and to what the tables
-        hold, and results do not depend on them.  Asynchronous on the context's stream."""
+        the most rows and the longest context of a sequence, choose how the work is cut, and with that the order of sums; they default to all rows
+        and to what the tables hold, and results are right whatever they say.  Asynchronous on the context's stream."""
         L, ctx = cache.layout, cache.ctx
         if L.head_dim != self.layout.head_dim or L.num_kv_heads != self.layout.num_kv_heads:
             _invalid("the cache is not of this attention's layout")
