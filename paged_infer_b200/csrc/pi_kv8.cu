@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32) kv8_write_kernel(const Write
   const long long job = (long long)blockIdx.x * kWriteWarps + warp;
   const int per_row = p.kv_heads * 2, hs = (int)(job % per_row), head = hs >> 1, side = hs & 1;
   const long long row0 = job / per_row * p.rows_per_warp;
+  pi_grid_dependency_wait();
   if (row0 >= p.n_rows) return;
   const void* src = side ? p.v : p.k;
   const size_t stride = side ? p.v_stride : p.k_stride, col = (size_t)head * p.head_dim;
@@ -266,8 +267,7 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
   const long long grid = (jobs + kWriteWarps - 1) / kWriteWarps;
   PI_REQUIRE(ctx, grid <= 0x7fffffffll, "too many rows");
   pi_prof_scope prof(ctx, PI_PROF_ROPE_KV);
-  if (pool->kind == PI_E4M3) kv8_write_kernel<PI_E4M3><<<(unsigned)grid, kWriteWarps * 32, 0, ctx->stream>>>(p);
-  else kv8_write_kernel<PI_INT8><<<(unsigned)grid, kWriteWarps * 32, 0, ctx->stream>>>(p);
+  PI_CUDA(ctx, pi_launch_chained(ctx, pool->kind == PI_E4M3 ? kv8_write_kernel<PI_E4M3> : kv8_write_kernel<PI_INT8>, dim3((unsigned)grid), dim3(kWriteWarps * 32), 0, 1, p));
   PI_CHECK_LAUNCH(ctx);
   return PI_OK;
 }

@@ -8,10 +8,14 @@
 // outputs, are two f16 planes (22 bits); those of bf16 and f16 outputs are one.  Queries are brought to [-1, 1] by a power of two
 // per column, weights to 2^14 at most, so that neither leaves f16's normal range; the scales stay in f32.
 //
-// Codes go from memory to registers without a shuffle: the k index of a product may be permuted at will, so a lane takes whole
-// words of a token's codes for K, and, for V, of the four tokens whose weights it holds; pairs of tokens are put together by byte
-// permutes.  The copies (cp.async) land where the same lane reads them, so a ring of tiles per warp needs no barrier.  Two 2 KB
-// tiles at pitch 128 are 8 copies a lane.
+// Codes go from memory straight to the registers that feed the products: the k index of a product may be permuted at will, so a
+// lane takes whole words of a token's codes for K, and, for V, of the four tokens whose weights it holds; pairs of tokens are put
+// together by byte permutes.  The next tile's K codes are requested as soon as this tile's are used up, its V codes likewise, so that
+// every warp has loads under way all the time without a second set of registers and without shared memory.
+//
+// int8 codes become f16 by a byte permute into the mantissa of 1024 (1024 + 128 + code).  With two planes the 1152 is subtracted from
+// every pair.  With one plane it stays in and the accumulators start from -1152 times the sum of the other operand instead: the sums
+// are 33 times larger than without, which costs 5 of the accumulator's 24 bits where the result has 8 or 11.
 //
 // The tokens of a sequence are dealt to the warps of a CTA and to the CTAs of a cluster; partial results are joined through shared
 // memory, then through the cluster's: no scratch in device memory, and the order of the sums is fixed.
@@ -26,14 +30,22 @@
 
 namespace pi_kv8 {
 
-constexpr int kWarpsD = 4, kStagesD = 4, kMaxSplit = 16;
-constexpr float kTopWeight = 14.f;   // log2 of what the largest weight is stored as
+constexpr int kMaxSplit = 16, kMaxWarps = 8;   // CTAs of a cluster, warps of a CTA
+// Weights are stored times 2^7 relative to a running maximum that may lag 2^8 behind: at most 2^15, below the largest f16, and
+// precise down to 2^-21 (one plane: of the largest).  The maximum is only taken across lanes when a score exceeds it by more.
+constexpr float kTopWeight = 7.f, kLag = 8.f;
 
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_from(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {   // d = a b + c, c the same for all rows
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // of an 8 x 8 tile of 16-bit values, a row per four lanes
   uint32_t y;
@@ -45,21 +57,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Codes are read once.
 template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
-template <int BYTES>
-__device__ __forceinline__ void load_words(uint32_t* to, const unsigned char* from) {
+__device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* from) {
   if constexpr (BYTES == 16) {
-    const uint4 v = *reinterpret_cast<const uint4*>(from);
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from));
     to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
   } else if constexpr (BYTES == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    const uint2 v = __ldcs(reinterpret_cast<const uint2*>(from));
     to[0] = v.x, to[1] = v.y;
   } else {
-    to[0] = *reinterpret_cast<const uint32_t*>(from);
+    to[0] = __ldcs(reinterpret_cast<const uint32_t*>(from));
   }
 }
 // How much a partial result (maximum, sum) counts beside the maximum of all: one that saw nothing does not, one that is not a
@@ -68,32 +76,25 @@ __device__ __forceinline__ float join_factor(float top, float sum, float all) {
   if (sum != sum) return sum;
   return top == -INFINITY ? 0.f : exp2_fast(top - all);
 }
-// Two codes as f16: bytes 0 and 1, or 2 and 3, of a word.  int8: 1024 + (code + 128) in the mantissa, less 1152.  e4m3: the bits of
-// 2^-8 times the value, subnormals included.
-template <int KIND>
-__device__ __forceinline__ uint32_t widen(uint32_t w, uint32_t sel_int8, uint32_t sel_e4m3) {
+// Two codes as f16: bytes 0 and 1, or 2 and 3, of a word.  int8 (its sign bit flipped): 1024 + (code + 128) in the mantissa, less 1152
+// unless that stays in.
+template <int KIND, bool BIASED>
+__device__ __forceinline__ uint32_t widen(uint32_t w, bool high) {
   if (KIND == PI_INT8) {
-    const uint32_t h = __byte_perm(w, 0x64646464u, sel_int8);
+    const uint32_t h = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
+    if (BIASED) return h;
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  const uint32_t h = __byte_perm(w, 0, sel_e4m3);
-  return (h & 0x80008000u) | (h >> 1 & 0x3f803f80u);
-}
-template <int KIND>
-__device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
-  return widen<KIND>(w, 0x4140, 0x1404);
-}
-template <int KIND>
-__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
-  return widen<KIND>(w, 0x4342, 0x3424);
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(high ? w >> 16 : w)));
+  return h;
 }
 template <int KIND>
 __device__ __forceinline__ uint32_t unsign(uint32_t w) {
   return KIND == PI_INT8 ? w ^ 0x80808080u : w;
 }
-template <int KIND>
-constexpr float kUnit = KIND == PI_INT8 ? 1.f : 256.f;   // what a widened code of 1 stands for
+constexpr float kBias = 1152.f;
 
 // f16 pair of two values and the pair of what is left.
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
@@ -112,393 +113,505 @@ struct Geometry {
   static constexpr int KB = PITCH % 64 == 0 ? 16 : 8, kpieces = PITCH / 4 / KB;
   // V: PITCH / 8 neighbouring channels of a token, in pieces of VB bytes
   static constexpr int VB = PITCH % 128 == 0 ? 16 : PITCH % 64 == 0 ? 8 : 4, vpieces = PITCH / 8 / VB;
-  static constexpr int stage = 2 * 16 * PITCH + 256;   // both tiles, and 8 bytes of scales a lane
 };
 
-template <int KIND, int PITCH, int PLANES, int NT>
+__device__ __forceinline__ uint32_t peer_addr(const void* mine, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(pi_mma::smem_addr(mine)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float2 peer2(const float2* mine, uint32_t rank) {   // the same variable of another CTA of the cluster
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_addr(mine, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer4(const float* mine, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_addr(mine, rank)) : "memory");
+  return v;
+}
+
+// Tiles that a warp works on at a time, and CTAs of eight warps that an SM has registers for: sixteen warps hide the chain from load
+// to product to exponential to product better than eight with longer steps (24 with 80 registers spill); wide heads and two groups
+// of columns leave room for eight.
+template <int PITCH, int NT>
+struct Shape {
+  static constexpr int TT = PITCH <= 64 && NT == 1 ? 2 : 1, min_ctas = PITCH <= 128 && NT == 1 ? 2 : 1, cols = 8 * NT;
+  static constexpr int line = PITCH + 4;   // floats between columns where warps meet
+};
+// Shared memory: query fragments, per column (first and last position seen, factor, bias), (max, sum) per warp, per CTA, partial results.
+template <int PITCH, int PLANES, int NT>
 struct Layout {
-  using G = Geometry<PITCH>;
   static constexpr int cols = 8 * NT;
-  static constexpr int ring = kWarpsD * kStagesD * G::stage;
-  static constexpr int queries = G::ksteps * PLANES * NT * 32 * 8;     // b fragments, 8 bytes a lane
-  static constexpr int merge = kWarpsD * cols * PITCH * 4 + kWarpsD * cols * 8;
-  static constexpr int body = ring > merge ? ring : merge;
-  static constexpr int bytes = body + queries + cols * 16 + cols * PITCH * 4 + cols * 8;
+  static constexpr int queries = PITCH / 16 * PLANES * NT * 32 * 8;     // b fragments, 8 bytes a lane
+  static constexpr int bytes(int warps) { return queries + cols * 16 + (warps + 1) * cols * 8 + (warps + 1) * cols * Shape<PITCH, NT>::line * 4; }
 };
 
 template <int KIND, int PITCH, int PLANES, int NT>
-__global__ void __launch_bounds__(kWarpsD * 32) kv8_decode_kernel(const pi_kv8_attn_params p) {
+__global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv8_decode_kernel(const pi_kv8_attn_params p) {
   using G = Geometry<PITCH>;
-  using S = Layout<KIND, PITCH, PLANES, NT>;
-  constexpr int COLS = S::cols;
+  using S = Shape<PITCH, NT>;
+  constexpr int COLS = S::cols, TT = S::TT, LINE = S::line;
+  constexpr bool BIASED = KIND == PI_INT8 && PLANES == 1;
   extern __shared__ __align__(16) unsigned char smem[];
-  unsigned char* s_queries = smem + S::body;
-  int* s_lo = reinterpret_cast<int*>(s_queries + S::queries);   // per column: first and last position seen, factor of the scores
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+  unsigned char* s_queries = smem;
+  int* s_lo = reinterpret_cast<int*>(smem + Layout<PITCH, PLANES, NT>::queries);
   int* s_hi = s_lo + COLS;
   float* s_factor = reinterpret_cast<float*>(s_hi + COLS);
-  float* s_out = s_factor + 2 * COLS;                           // this CTA's result [column][pitch], then (max, sum) per column
-  float* s_stat = s_out + COLS * PITCH;
+  float* s_bias = s_factor + COLS;
+  float2* s_stat = reinterpret_cast<float2*>(s_bias + COLS);   // of the CTA
+  float2* s_warp = s_stat + COLS;                              // [warp][column]
+  float* s_out = reinterpret_cast<float*>(s_warp + warps * COLS);   // [column][line] of the CTA
+  float* s_part = s_out + COLS * LINE;                         // [warp][column][line]
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint32_t split, splits;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const int kvh = blockIdx.x / splits, seq = blockIdx.y, bs = p.block_size;
+  pi_grid_dependency_wait();
   const int row_begin = max(0, min(p.cu_rows[seq], p.n_rows)), row_end = min(p.cu_rows[seq + 1], p.n_rows);
   const int ncols = (row_end - row_begin) * p.group;
+  const int last_token = (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1;
+  const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
   // one tile of columns as the grid is cut; the loop is for sequences that bring more rows than the call said
   for (int col0 = blockIdx.z * COLS; col0 < ncols; col0 += gridDim.z * COLS) {
-  // columns: what they see, and their queries as b fragments
-  int lo_all = 0x7fffffff, hi_all = -1;
-  for (int c = tid; c < COLS; c += kWarpsD * 32) {
-    int lo = 0x7fffffff, hi = -1;
-    if (col0 + c < ncols) {
-      const int pos = p.row_pos[row_begin + (col0 + c) / p.group];
-      lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
-      hi = pos;
+    // what the tile's columns see
+    int lo_all = 0x7fffffff, hi_all = -1, lo_most = 0, hi_least = 0x7fffffff;
+    const int first_row = row_begin + p.by_group(col0), last_row = row_begin + p.by_group(min(ncols, col0 + COLS) - 1);
+    for (int r = first_row; r <= last_row; ++r) {
+      const int pos = p.row_pos[r], from = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+      if (pos >= 0) lo_all = min(lo_all, from);
+      hi_all = max(hi_all, pos);
+      lo_most = max(lo_most, from);
+      hi_least = min(hi_least, pos);
     }
-    s_lo[c] = lo;
-    s_hi[c] = hi;
-  }
-  // a warp per column: the power of two that brings its query to [-1, 1]
-  for (int c = warp; c < COLS; c += kWarpsD) {
-    float top = 0.f, x[(PITCH + 31) / 32];
-    const bool live = col0 + c < ncols;
-    const size_t at = live ? (size_t)(row_begin + (col0 + c) / p.group) * p.q_stride + (size_t)(kvh * p.group + (col0 + c) % p.group) * p.head_dim : 0;
-#pragma unroll
-    for (int i = 0; i < (PITCH + 31) / 32; ++i) {
-      const int d = lane + 32 * i;
-      x[i] = live && d < p.head_dim ? pi_load_as_f32(p.q, at + d, p.dtype) : 0.f;
-      top = fmaxf(top, fabsf(x[i]));
-    }
-    top = pi_warp_max(top);
-    // exponent e with 2^(e-1) <= top < 2^e; 2^e and 2^-e both have to be f32
-    const int e = top > 0.f && top < INFINITY ? min(max(ilogbf(top) + 1, -126), 126) : 0;
-    const float shrink = scalbnf(1.f, -e);
-    if (lane == 0) s_factor[c] = scalbnf(1.f, e) * p.scale2;
-#pragma unroll
-    for (int i = 0; i < (PITCH + 31) / 32; ++i) {
-      const int d = lane + 32 * i;
-      if (d >= PITCH) continue;
-      // channel d is byte b of word j of lane tt
-      const int piece = d / (G::KB * 4), in = d % (G::KB * 4), tt = in / G::KB, j = piece * (G::KB / 4) + in % G::KB / 4, b = d & 3;
-      const float v = x[i] * shrink;
-      const __half hi = __float2half_rn(v);
-#pragma unroll
-      for (int pl = 0; pl < PLANES; ++pl) {
-        __half* f = reinterpret_cast<__half*>(s_queries + ((((size_t)j * PLANES + pl) * NT + c / 8) * 32 + (c % 8) * 4 + tt) * 8);
-        f[b] = pl == 0 ? hi : __float2half_rn(v - __half2float(hi));
-      }
-    }
-  }
-  __syncthreads();
-  for (int c = 0; c < COLS; ++c)
-    if (s_hi[c] >= 0) {
-      lo_all = min(lo_all, s_lo[c]);
-      hi_all = max(hi_all, s_hi[c]);
-    }
-  hi_all = min(hi_all, (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1);
+    hi_all = min(hi_all, last_token);
+    hi_least = min(hi_least, hi_all);
 
-  // tiles: 16 tokens of a block, dealt to the warps of all CTAs in turn
-  const int per_block = (bs + 15) / 16;
-  const int first_block = lo_all / bs, tiles = hi_all < lo_all ? 0 : (hi_all / bs - first_block + 1) * per_block;
-  const int worker = (int)split * kWarpsD + warp, workers = (int)splits * kWarpsD;
-  const int mine = tiles > worker ? (tiles - worker + workers - 1) / workers : 0;
-  const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
-  const uint32_t ring = pi_mma::smem_addr(smem) + (uint32_t)warp * kStagesD * G::stage;
-  const size_t tile_bytes = (size_t)bs * PITCH;
-
-  auto tile_block = [&](int i) -> int {   // the physical block of this warp's tile i, -1: not mapped
-    if (i >= mine) return -1;
-    const int b = __ldg(table + first_block + (worker + i * workers) / per_block);
-    return b < p.num_blocks ? b : -1;
-  };
-  auto request = [&](int i, int block) {
-    if (block >= 0) {
-      const int sub = (worker + i * workers) % per_block * 16;
-      const size_t tile = ((size_t)block * p.kv_heads + kvh) * 2;
-      const uint8_t* k = p.codes + tile * tile_bytes;
-      const uint8_t* v = k + tile_bytes;
-      const uint32_t to = ring + (uint32_t)(i % kStagesD) * G::stage;
+    // tiles: 16 tokens of a block; rounds of TT neighbouring ones are dealt to the warps of all CTAs in turn
+    const int per_block = (bs + 15) >> 4;
+    const int first_block = hi_all < lo_all ? 0 : p.by_block(lo_all), blocks = hi_all < lo_all ? 0 : p.by_block(hi_all) - first_block + 1;
+    const int workers = (int)splits * warps, step_block = p.by_tiles(TT * workers), step_sub = TT * workers - step_block * per_block;
+    int block[TT], sub[TT];   // of the tiles to look up next: from the first block, in the block
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint8_t* row = k + (size_t)min(sub + g + 8 * r, bs - 1) * PITCH + t * G::KB;
-#pragma unroll
-        for (int c = 0; c < G::kpieces; ++c) copy_async<G::KB>(to + ((r * G::kpieces + c) * 32 + lane) * G::KB, row + c * G::KB * 4);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint8_t* row = v + (size_t)min(sub + 2 * t + (r & 1) + (r & 2) * 4, bs - 1) * PITCH + g * (PITCH / 8);
-#pragma unroll
-        for (int c = 0; c < G::vpieces; ++c) copy_async<G::VB>(to + 16 * PITCH + ((r * G::vpieces + c) * 32 + lane) * G::VB, row + c * G::VB);
-      }
-      copy_async<8>(to + 32 * PITCH + lane * 8, p.scales + tile);
+    for (int e = 0; e < TT; ++e) {
+      const int first = TT * ((int)split * warps + warp) + e;
+      block[e] = p.by_tiles(first);
+      sub[e] = first - block[e] * per_block;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-
-  float out[NT][G::mtiles][4], top[NT][2], sum[NT][2], factor[NT][2];
-  int lo[NT][2], hi[NT][2];
+    int next_id[TT], next_base[TT], next_sub[TT];   // looked up: physical block (-1: none), first token, place in the block
+    auto look = [&]() {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int c = n * 8 + 2 * t + e;
-      top[n][e] = -INFINITY;
-      sum[n][e] = 0.f;
-      factor[n][e] = s_factor[c];
-      lo[n][e] = s_lo[c];
-      hi[n][e] = min(s_hi[c], hi_all);
-    }
-#pragma unroll
-    for (int m = 0; m < G::mtiles; ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[n][m][e] = 0.f;
-  }
-
-  int blocks[kStagesD];
-#pragma unroll
-  for (int i = 0; i < kStagesD - 1; ++i) {
-    blocks[i] = tile_block(i);
-    request(i, blocks[i]);
-  }
-  int ahead = tile_block(kStagesD - 1);
-  for (int i = 0; i < mine; ++i) {
-    blocks[kStagesD - 1] = ahead;
-    request(i + kStagesD - 1, ahead);
-    ahead = tile_block(i + kStagesD);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStagesD - 1) : "memory");
-    const int block = blocks[0];
-#pragma unroll
-    for (int k = 0; k < kStagesD - 1; ++k) blocks[k] = blocks[k + 1];
-    if (block < 0) continue;
-    const unsigned char* at = smem + (size_t)warp * kStagesD * G::stage + (size_t)(i % kStagesD) * G::stage;
-    const int tile = worker + i * workers, sub = tile % per_block * 16;
-    const int base = (first_block + tile / per_block) * bs + sub, valid = min(16, bs - sub);
-    const float2 scale = *reinterpret_cast<const float2*>(at + 32 * PITCH + lane * 8);
-
-    float s[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-    {
-      uint32_t kw[2][PITCH / 16];
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int c = 0; c < G::kpieces; ++c) {
-          const unsigned char* from = at + ((r * G::kpieces + c) * 32 + lane) * G::KB;
-          load_words<G::KB>(&kw[r][c * G::KB / 4], from);
+      for (int e = 0; e < TT; ++e) {
+        next_id[e] = -1;
+        if (block[e] < blocks) next_id[e] = __ldg(table + first_block + block[e]);
+        next_sub[e] = sub[e] * 16;
+        next_base[e] = (first_block + block[e]) * bs + sub[e] * 16;
+        block[e] += step_block;
+        sub[e] += step_sub;
+        if (sub[e] >= per_block) {
+          sub[e] -= per_block;
+          ++block[e];
         }
+      }
+    };
+    const bool whole = (bs & 15) == 0;   // no tile reaches beyond its block
+    const uint8_t* k_lane = p.codes + (size_t)kvh * 2 * p.side_bytes + t * G::KB;
+    const uint8_t* v_lane = p.codes + ((size_t)kvh * 2 + 1) * p.side_bytes + g * (PITCH / 8);
+    const float* scale_head = p.scales + kvh * 2;
+
+    uint32_t kw[TT][2][PITCH / 16], vw[TT][4][PITCH / 32];
+    float2 k_scale[TT];       // both scales of the tile whose K codes are in kw
+    int id[TT], base[TT], place[TT];
+    auto load_k = [&]() {     // of the tiles that were looked up last
+#pragma unroll
+      for (int e = 0; e < TT; ++e) {
+        id[e] = (uint32_t)next_id[e] < (uint32_t)p.num_blocks ? next_id[e] : -1;
+        base[e] = next_base[e];
+        place[e] = next_sub[e];
+        k_scale[e] = make_float2(0.f, 0.f);
+        if (id[e] >= 0) {
+          k_scale[e] = __ldg(reinterpret_cast<const float2*>(scale_head + (unsigned long long)(uint32_t)id[e] * (uint32_t)(p.kv_heads * 2)));
+          const uint8_t* k = k_lane + (unsigned long long)(uint32_t)id[e] * p.block_bytes;
+          if (whole) {
+            k += (place[e] + g) * PITCH;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int c = 0; c < G::kpieces; ++c) load_words<G::KB>(&kw[e][r][c * G::KB / 4], k + r * 8 * PITCH + c * G::KB * 4);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int c = 0; c < G::kpieces; ++c) load_words<G::KB>(&kw[e][r][c * G::KB / 4], k + min(place[e] + g + 8 * r, bs - 1) * PITCH + c * G::KB * 4);
+          }
+        }
+      }
+    };
+    auto load_v = [&]() {     // of the tiles whose K codes were requested last
+#pragma unroll
+      for (int e = 0; e < TT; ++e)
+        if (id[e] >= 0) {
+          const uint8_t* v = v_lane + (unsigned long long)(uint32_t)id[e] * p.block_bytes;
+          if (whole) {
+            v += (place[e] + 2 * t) * PITCH;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int c = 0; c < G::vpieces; ++c) load_words<G::VB>(&vw[e][r][c * G::VB / 4], v + ((r & 1) + (r & 2) * 4) * PITCH + c * G::VB);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int c = 0; c < G::vpieces; ++c)
+                load_words<G::VB>(&vw[e][r][c * G::VB / 4], v + min(place[e] + 2 * t + (r & 1) + (r & 2) * 4, bs - 1) * PITCH + c * G::VB);
+          }
+        }
+    };
+    const int tiles = blocks * per_block, rounds = (tiles + TT - 1) / TT, worker = (int)split * warps + warp;
+    int mine = rounds > worker ? p.by_workers(rounds - worker - 1) + 1 : 0;
+    look();
+    load_k();
+    load_v();
+    look();
+
+    // the first codes are under way; meanwhile the columns' queries become b fragments: eight lanes a column, four channels at a time,
+    // each column times the power of two that brings it to [-1, 1]
+    for (int c = tid >> 3; c < COLS; c += warps * 4) {
+      const int l8 = lane & 7, rel = col0 + c < ncols ? p.by_group(col0 + c) : 0, row = row_begin + rel;
+      const bool live = col0 + c < ncols;
+      const size_t at = (size_t)row * p.q_stride + (size_t)(kvh * p.group + (col0 + c - rel * p.group)) * p.head_dim;
+      float x[PITCH / 32][4], most = 0.f;
+#pragma unroll
+      for (int i = 0; i < PITCH / 32; ++i) {
+        const int d = 4 * (l8 + 8 * i);
+        pi_load4_as_f32(x[i], p.q, at + d, p.dtype, live ? p.head_dim - d : 0, p.q_wide);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) most = fmaxf(most, fabsf(x[i][b]));
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      // 2^(e - 127) <= most < 2^(e - 126); both powers below stay normal
+      const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);
+      const float shrink = __uint_as_float((253u - e) << 23);   // 2^(126 - e)
+      float bias = 0.f;
+#pragma unroll
+      for (int i = 0; i < PITCH / 32; ++i) {
+        const int d = 4 * (l8 + 8 * i), piece = d / (G::KB * 4), in = d % (G::KB * 4), to = (piece * (G::KB / 4) + in % G::KB / 4) * PLANES;
+        float y[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) y[b] = x[i][b] * shrink;
+        uint2 hi = make_uint2(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]));
+        uint2* frag = reinterpret_cast<uint2*>(s_queries) + ((size_t)to * NT + c / 8) * 32 + (c % 8) * 4 + in / G::KB;
+        frag[0] = hi;
+        if constexpr (PLANES == 2) frag[NT * 32] = make_uint2(pack_rest(y[0], y[1], hi.x), pack_rest(y[2], y[3], hi.y));
+        if constexpr (BIASED) {
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+          bias += (a.x + a.y) + (b.x + b.y);
+        }
+      }
+      if constexpr (BIASED) {
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) bias += __shfl_xor_sync(0xffffffffu, bias, o);
+      }
+      if (l8 == 0) {
+        const int pos = live ? p.row_pos[row] : -1;
+        s_lo[c] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+        s_hi[c] = pos;
+        s_factor[c] = __uint_as_float((e + 1) << 23) * p.scale2;   // 2^(e - 126)
+        s_bias[c] = -kBias * bias;
+      }
+    }
+    __syncthreads();
+
+    float out[NT][G::mtiles][4], top[NT][2], sum[NT][2], factor[NT][2], q_bias[NT][2];
+    int lo[NT][2], hi[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = n * 8 + 2 * t + e;
+        top[n][e] = -INFINITY;
+        sum[n][e] = 0.f;
+        factor[n][e] = s_factor[c];
+        q_bias[n][e] = BIASED ? s_bias[c] : 0.f;
+        lo[n][e] = s_lo[c];
+        hi[n][e] = min(s_hi[c], hi_all);
+      }
+#pragma unroll
+      for (int m = 0; m < G::mtiles; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[n][m][e] = 0.f;
+    }
+
+    for (; mine > 0; --mine) {
+      int valid[TT], token[TT];
+      float2 scale[TT];
+      bool all = true;   // every column sees every token
+#pragma unroll
+      for (int e = 0; e < TT; ++e) {
+        valid[e] = id[e] >= 0 ? min(16, bs - place[e]) : 0;
+        token[e] = base[e];
+        all = all && valid[e] == 16 && token[e] >= lo_most && token[e] + 15 <= hi_least;
+        scale[e] = k_scale[e];
+      }
+      if constexpr (KIND == PI_E4M3) {
+        // bytes of tokens that nobody sees may be anything, also what e4m3 calls NaN; a weight of zero does not silence that
+        if (!all) {
+#pragma unroll
+          for (int e = 0; e < TT; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = 2 * t + (r & 1) + (r & 2) * 4;
+              const bool seen = row < valid[e] && token[e] + row >= lo_all && token[e] + row <= hi_all;
+#pragma unroll
+              for (int w = 0; w < PITCH / 32; ++w) vw[e][r][w] = seen ? vw[e][r][w] : 0;
+            }
+        }
+      }
+      float s[TT][NT][4];
 #pragma unroll
       for (int j = 0; j < G::ksteps; ++j) {
-        const uint32_t w0 = unsign<KIND>(kw[0][j]), w1 = unsign<KIND>(kw[1][j]);
-        const uint32_t a0 = widen_lo<KIND>(w0), a1 = widen_lo<KIND>(w1), a2 = widen_hi<KIND>(w0), a3 = widen_hi<KIND>(w1);
+        uint32_t a[TT][4];
+#pragma unroll
+        for (int e = 0; e < TT; ++e) {
+          const uint32_t w0 = unsign<KIND>(kw[e][0][j]), w1 = unsign<KIND>(kw[e][1][j]);
+          a[e][0] = widen<KIND, BIASED>(w0, false);
+          a[e][1] = widen<KIND, BIASED>(w1, false);
+          a[e][2] = widen<KIND, BIASED>(w0, true);
+          a[e][3] = widen<KIND, BIASED>(w1, true);
+        }
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint2 b = *reinterpret_cast<const uint2*>(s_queries + (((size_t)j * PLANES + pl) * NT + n) * 256 + lane * 8);
-            mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
+            const uint2 b = reinterpret_cast<const uint2*>(s_queries)[((j * PLANES + pl) * NT + n) * 32 + lane];
+#pragma unroll
+            for (int e = 0; e < TT; ++e) {
+              if (j == 0 && pl == 0) mma_f16_from(s[e][n], a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y, q_bias[n][0], q_bias[n][1]);
+              else mma_f16(s[e][n], a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y);
+            }
           }
       }
-    }
+      load_k();   // of the next round; the table's entries for the one behind it are on their way a whole round ahead
+      look();
 
-    // softmax of the tile: this lane has tokens g and g + 8 of columns 2 t and 2 t + 1
-    uint32_t pw[NT][2][PLANES];
-    bool part = !(scale.y < INFINITY);
+      // softmax: this lane has tokens g and g + 8 of every tile, columns 2 t and 2 t + 1
+      uint32_t pw[TT][NT][2][PLANES];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float most[2], shrink[2];
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float f = factor[n][e] * (scale.x * kUnit<KIND>);
-        const int t0 = base + g, t1 = t0 + 8;
-        s[n][e] = t0 >= lo[n][e] && t0 <= hi[n][e] && g < valid ? s[n][e] * f : -INFINITY;
-        s[n][2 + e] = t1 >= lo[n][e] && t1 <= hi[n][e] && g + 8 < valid ? s[n][2 + e] * f : -INFINITY;
-        most[e] = fmaxf(s[n][e], s[n][2 + e]);
-      }
+        for (int e = 0; e < TT; ++e)
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], o));
-        most[1] = fmaxf(most[1], __shfl_xor_sync(0xffffffffu, most[1], o));
-      }
-      bool grown = false;
+          for (int c = 0; c < 2; ++c) {
+            const float f = factor[n][c] * scale[e].x;
+            s[e][n][c] *= f;
+            s[e][n][2 + c] *= f;
+          }
+        if (!all) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float now = fmaxf(top[n][e], most[e]), zero = now == -INFINITY ? 0.f : now;
-        shrink[e] = exp2_fast(top[n][e] - zero);
-        grown |= now != top[n][e];
-        top[n][e] = now;
-        s[n][e] = exp2_fast(s[n][e] - zero + kTopWeight);
-        s[n][2 + e] = exp2_fast(s[n][2 + e] - zero + kTopWeight);
-        sum[n][e] = sum[n][e] * shrink[e] + (s[n][e] + s[n][2 + e]);
-      }
-      if (__any_sync(0xffffffffu, grown)) {
+          for (int e = 0; e < TT; ++e)
 #pragma unroll
-        for (int m = 0; m < G::mtiles; ++m) {
-          out[n][m][0] *= shrink[0];
-          out[n][m][1] *= shrink[1];
-          out[n][m][2] *= shrink[0];
-          out[n][m][3] *= shrink[1];
+            for (int c = 0; c < 4; ++c) {
+              const int row = g + (c >> 1) * 8, at_token = token[e] + row;
+              if (row >= valid[e] || at_token < lo[n][c & 1] || at_token > hi[n][c & 1]) s[e][n][c] = -INFINITY;
+            }
         }
+        float most[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          most[c] = fmaxf(s[0][n][c], s[0][n][2 + c]);
+#pragma unroll
+          for (int e = 1; e < TT; ++e) most[c] = fmaxf(most[c], fmaxf(s[e][n][c], s[e][n][2 + c]));
+        }
+        // the first scores of a column exceed minus infinity by more than any lag
+        if (__any_sync(0xffffffffu, most[0] > top[n][0] + kLag || most[1] > top[n][1] + kLag)) {
+          float shrink[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], o));
+            const float now = fmaxf(top[n][c], most[c]);
+            shrink[c] = exp2_fast(top[n][c] - (now == -INFINITY ? 0.f : now));
+            top[n][c] = now;
+            sum[n][c] *= shrink[c];
+          }
+#pragma unroll
+          for (int m = 0; m < G::mtiles; ++m) {
+            out[n][m][0] *= shrink[0];
+            out[n][m][1] *= shrink[1];
+            out[n][m][2] *= shrink[0];
+            out[n][m][3] *= shrink[1];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float from = (top[n][c] == -INFINITY ? 0.f : top[n][c]) - kTopWeight;
+#pragma unroll
+          for (int e = 0; e < TT; ++e) {
+            s[e][n][c] = exp2_fast(s[e][n][c] - from);
+            s[e][n][2 + c] = exp2_fast(s[e][n][2 + c] - from);
+            sum[n][c] += s[e][n][c] + s[e][n][2 + c];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < TT; ++e)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t h = pack_f16(s[e][n][2 * r], s[e][n][2 * r + 1]);
+            pw[e][n][r][0] = transpose8(h);
+            if constexpr (PLANES == 2) pw[e][n][r][1] = transpose8(pack_rest(s[e][n][2 * r], s[e][n][2 * r + 1], h));
+          }
       }
-      const uint32_t h0 = pack_f16(s[n][0], s[n][1]), h1 = pack_f16(s[n][2], s[n][3]);
-      pw[n][0][0] = transpose8(h0);
-      pw[n][1][0] = transpose8(h1);
-      if constexpr (PLANES == 2) {
-        pw[n][0][1] = transpose8(pack_rest(s[n][0], s[n][1], h0));
-        pw[n][1][1] = transpose8(pack_rest(s[n][2], s[n][3], h1));
-      }
-    }
 
-    const float unit = scale.y * kUnit<KIND>;
-    uint32_t vw[4][PITCH / 32];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int c = 0; c < G::vpieces; ++c) {
-        const unsigned char* from = at + 16 * PITCH + ((r * G::vpieces + c) * 32 + lane) * G::VB;
-        load_words<G::VB>(&vw[r][c * G::VB / 4], from);
-      }
-#pragma unroll
-    for (int w = 0; w < PITCH / 32; ++w) {
-      const uint32_t v0 = unsign<KIND>(vw[0][w]), v1 = unsign<KIND>(vw[1][w]), v2 = unsign<KIND>(vw[2][w]), v3 = unsign<KIND>(vw[3][w]);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t x = __byte_perm(v0, v1, half ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, half ? 0x7362 : 0x5140);
-        const uint32_t a0 = widen_lo<KIND>(x), a1 = widen_hi<KIND>(x), a2 = widen_lo<KIND>(y), a3 = widen_hi<KIND>(y);
+      for (int e = 0; e < TT; ++e) {
+        // the V scale per column; one that is not finite reaches the columns that see the tile and no others
+        float unit[NT][2], p_bias[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int pl = 0; pl < PLANES; ++pl) mma_f16(d, a0, a1, a2, a3, pw[n][0][pl], pw[n][1][pl]);
-          float* o = out[n][2 * w + half];
-          if (!part) {
+          for (int c = 0; c < 2; ++c) {
+            unit[n][c] = all || (token[e] + valid[e] > lo[n][c] && token[e] <= hi[n][c] && valid[e] > 0) ? scale[e].y : 0.f;
+            p_bias[n][c] = 0.f;
+          }
+          if constexpr (BIASED) {   // the sum of the weights as they were rounded: a product with ones
+            float d[4];
+            constexpr uint32_t ones = 0x3c003c00u;
+            mma_f16_from(d, ones, ones, ones, ones, pw[e][n][0][0], pw[e][n][1][0], 0.f, 0.f);
+            p_bias[n][0] = -kBias * d[0];
+            p_bias[n][1] = -kBias * d[1];
+          }
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(unit, d[e], o[e]);
-          } else {   // values that are not finite reach the columns that see them and no others
+        for (int w = 0; w < PITCH / 32; ++w) {
+          const uint32_t v0 = unsign<KIND>(vw[e][0][w]), v1 = unsign<KIND>(vw[e][1][w]), v2 = unsign<KIND>(vw[e][2][w]), v3 = unsign<KIND>(vw[e][3][w]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (base + valid > lo[n][e & 1] && base <= hi[n][e & 1]) o[e] = fmaf(unit, d[e], o[e]);
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(v0, v1, half ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, half ? 0x7362 : 0x5140);
+            const uint32_t a0 = widen<KIND, BIASED>(x, false), a1 = widen<KIND, BIASED>(x, true), a2 = widen<KIND, BIASED>(y, false), a3 = widen<KIND, BIASED>(y, true);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float d[4];
+              mma_f16_from(d, a0, a1, a2, a3, pw[e][n][0][0], pw[e][n][1][0], p_bias[n][0], p_bias[n][1]);
+              if constexpr (PLANES == 2) mma_f16(d, a0, a1, a2, a3, pw[e][n][0][1], pw[e][n][1][1]);
+              float* o = out[n][2 * w + half];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[c] = fmaf(unit[n][c & 1], d[c], o[c]);
+            }
           }
         }
       }
+      load_v();
     }
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();   // the ring becomes the place where the warps' results meet
 
-  float* s_part = reinterpret_cast<float*>(smem);                    // [warp][column][pitch]
-  float2* s_warp = reinterpret_cast<float2*>(s_part + kWarpsD * COLS * PITCH);   // (max, sum) [warp][column]
+    // the warps' results meet: a common maximum, then sums in the order of the warps
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float l = sum[n][e];
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      const int c = n * 8 + 2 * t + e;
-      if (g == 0) s_warp[warp * COLS + c] = make_float2(top[n][e], l);
-#pragma unroll
-      for (int m = 0; m < G::mtiles; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) s_part[((size_t)warp * COLS + c) * PITCH + g * (PITCH / 8) + 2 * m + r] = out[n][m][2 * r + e];
-    }
-  __syncthreads();
-  // the CTA's result, not yet divided by its sum
-  for (int i = tid; i < COLS * PITCH; i += kWarpsD * 32) {
-    const int c = i / PITCH;
-    float m = -INFINITY, v = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarpsD; ++w) m = fmaxf(m, s_warp[w * COLS + c].x);
-#pragma unroll
-    for (int w = 0; w < kWarpsD; ++w) {
-      const float2 st = s_warp[w * COLS + c];
-      const float f = join_factor(st.x, st.y, m);
-      if (f != 0.f) {
-        v = fmaf(f, s_part[(size_t)w * COLS * PITCH + i], v);
-        l = fmaf(f, st.y, l);
+        for (int o = 4; o < 32; o <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
+        if (g == 0) s_warp[warp * COLS + n * 8 + 2 * t + e] = make_float2(top[n][e], sum[n][e]);
       }
-    }
-    s_out[i] = v;
-    if (i % PITCH == 0) {
-      s_stat[2 * c] = m;
-      s_stat[2 * c + 1] = l;
-    }
-  }
-  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  else __syncthreads();
-
-  auto peer = [&](const float* mine_at, uint32_t rank) -> float {
-    uint32_t a;
-    float v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(pi_mma::smem_addr(mine_at)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-  };
-  // every CTA of the cluster finishes its share of the columns' channels
-  const int live = min(COLS, ncols - col0), total = live * PITCH, share = (total + (int)splits - 1) / (int)splits;
-  for (int i = (int)split * share + tid; i < min(total, ((int)split + 1) * share); i += kWarpsD * 32) {
-    const int c = i / PITCH, d = i % PITCH;
-    if (d >= p.head_dim) continue;
-    float m = -INFINITY, v = 0.f, l = 0.f;
-    for (uint32_t r = 0; r < splits; ++r) m = fmaxf(m, peer(s_stat + 2 * c, r));
-    for (uint32_t r = 0; r < splits; ++r) {
-      const float lr = peer(s_stat + 2 * c + 1, r), f = join_factor(peer(s_stat + 2 * c, r), lr, m);
-      if (f != 0.f) {
-        v = fmaf(f, peer(s_out + i, r), v);
-        l = fmaf(f, lr, l);
+    __syncthreads();
+    if (tid < COLS) {
+      float m = -INFINITY, l = 0.f;
+      for (int w = 0; w < warps; ++w) m = fmaxf(m, s_warp[w * COLS + tid].x);
+      for (int w = 0; w < warps; ++w) {
+        const float2 st = s_warp[w * COLS + tid];
+        l = fmaf(join_factor(st.x, st.y, m), st.y, l);
       }
+      s_stat[tid] = make_float2(m, l);
     }
-    const int row = row_begin + (col0 + c) / p.group, head = kvh * p.group + (col0 + c) % p.group;
-    pi_store_f32_as(p.out, (size_t)row * p.out_stride + (size_t)head * p.head_dim + d, p.dtype, l == 0.f ? 0.f : v / l);
-  }
-  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  else __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = n * 8 + 2 * t + e;
+        float m = -INFINITY;
+        for (int w = 0; w < warps; ++w) m = fmaxf(m, s_warp[w * COLS + c].x);
+        const float f = join_factor(top[n][e], sum[n][e], m);
+        float* to = s_part + (warp * COLS + c) * LINE + g * (PITCH / 8);
+#pragma unroll
+        for (int i = 0; i < PITCH / 32; ++i)
+          *reinterpret_cast<float4*>(to + 4 * i) = make_float4(out[n][2 * i][e] * f, out[n][2 * i][2 + e] * f, out[n][2 * i + 1][e] * f, out[n][2 * i + 1][2 + e] * f);
+      }
+    __syncthreads();
+    const int live = min(COLS, ncols - col0);
+    auto store = [&](int c, int d, float4 v, float l) {
+      const int rel = p.by_group(col0 + c);
+      const float inv = l == 0.f ? 0.f : 1.f / l, y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+      pi_store4_f32_as(y, p.out, (size_t)(row_begin + rel) * p.out_stride + (size_t)(kvh * p.group + (col0 + c - rel * p.group)) * p.head_dim + d, p.dtype, p.head_dim - d, p.out_wide);
+    };
+    for (int i = tid; i < live * (PITCH / 4); i += warps * 32) {
+      const int c = i / (PITCH / 4), d = i % (PITCH / 4) * 4;
+      float4 v = *reinterpret_cast<const float4*>(s_part + c * LINE + d);
+      for (int w = 1; w < warps; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(s_part + (w * COLS + c) * LINE + d);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      if (splits > 1) *reinterpret_cast<float4*>(s_out + c * LINE + d) = v;
+      else if (d < p.head_dim) store(c, d, v, s_stat[c].y);
+    }
+    if (splits > 1) {
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      // every CTA of the cluster finishes its share of the columns' channels
+      const int total = live * (PITCH / 4), share = (total + (int)splits - 1) / (int)splits;
+      for (int i = (int)split * share + tid; i < min(total, ((int)split + 1) * share); i += warps * 32) {
+        const int c = i / (PITCH / 4), d = i % (PITCH / 4) * 4;
+        if (d >= p.head_dim) continue;
+        float m = -INFINITY, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t r = 0; r < splits; ++r) m = fmaxf(m, peer2(s_stat + c, r).x);
+        for (uint32_t r = 0; r < splits; ++r) {
+          const float2 st = peer2(s_stat + c, r);
+          const float4 x = peer4(s_out + c * LINE + d, r);
+          const float f = join_factor(st.x, st.y, m);
+          v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+          l = fmaf(f, st.y, l);
+        }
+        store(c, d, v, l);
+      }
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+      __syncthreads();
+    }
   }
 }
 
 template <int KIND, int PITCH, int PLANES, int NT>
-pi_status launch_decode(pi_ctx* ctx, const pi_kv8_attn_params& p, dim3 grid, int splits) {
-  constexpr int bytes = Layout<KIND, PITCH, PLANES, NT>::bytes;
+pi_status launch_decode(pi_ctx* ctx, const pi_kv8_attn_params& p, dim3 grid, int splits, int warps) {
+  static_assert(Layout<PITCH, PLANES, NT>::bytes(kMaxWarps) <= 227 * 1024, "shared memory");
+  const int bytes = Layout<PITCH, PLANES, NT>::bytes(warps);
   auto kernel = kv8_decode_kernel<KIND, PITCH, PLANES, NT>;
   static pi_smem_grant grant;
-  if (grant.of(ctx) < (size_t)bytes) {
-    PI_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (grant.of(ctx) == 0) {
+    constexpr int most = Layout<PITCH, PLANES, NT>::bytes(kMaxWarps);
+    PI_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     PI_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    grant.of(ctx) = bytes;
+    grant.of(ctx) = most;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kWarpsD * 32);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)splits, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  PI_CUDA(ctx, cudaLaunchKernelEx(&cfg, kernel, p));
+  PI_CUDA(ctx, pi_launch_chained(ctx, kernel, grid, dim3(warps * 32), bytes, splits, p));
   PI_CHECK_LAUNCH(ctx);
   return PI_OK;
 }
 
 template <int PITCH>
-pi_status launch_decode_pitch(pi_ctx* ctx, int kind, int planes, int nt, const pi_kv8_attn_params& p, dim3 grid, int splits) {
+pi_status launch_decode_pitch(pi_ctx* ctx, int kind, int planes, int nt, const pi_kv8_attn_params& p, dim3 grid, int splits, int warps) {
   if (kind == PI_INT8) {
-    if (planes == 2) return nt == 1 ? launch_decode<PI_INT8, PITCH, 2, 1>(ctx, p, grid, splits) : launch_decode<PI_INT8, PITCH, 2, 2>(ctx, p, grid, splits);
-    return nt == 1 ? launch_decode<PI_INT8, PITCH, 1, 1>(ctx, p, grid, splits) : launch_decode<PI_INT8, PITCH, 1, 2>(ctx, p, grid, splits);
+    if (planes == 2) return nt == 1 ? launch_decode<PI_INT8, PITCH, 2, 1>(ctx, p, grid, splits, warps) : launch_decode<PI_INT8, PITCH, 2, 2>(ctx, p, grid, splits, warps);
+    return nt == 1 ? launch_decode<PI_INT8, PITCH, 1, 1>(ctx, p, grid, splits, warps) : launch_decode<PI_INT8, PITCH, 1, 2>(ctx, p, grid, splits, warps);
   }
-  if (planes == 2) return nt == 1 ? launch_decode<PI_E4M3, PITCH, 2, 1>(ctx, p, grid, splits) : launch_decode<PI_E4M3, PITCH, 2, 2>(ctx, p, grid, splits);
-  return nt == 1 ? launch_decode<PI_E4M3, PITCH, 1, 1>(ctx, p, grid, splits) : launch_decode<PI_E4M3, PITCH, 1, 2>(ctx, p, grid, splits);
+  if (planes == 2) return nt == 1 ? launch_decode<PI_E4M3, PITCH, 2, 1>(ctx, p, grid, splits, warps) : launch_decode<PI_E4M3, PITCH, 2, 2>(ctx, p, grid, splits, warps);
+  return nt == 1 ? launch_decode<PI_E4M3, PITCH, 1, 1>(ctx, p, grid, splits, warps) : launch_decode<PI_E4M3, PITCH, 1, 2>(ctx, p, grid, splits, warps);
 }
-extern template pi_status launch_decode_pitch<32>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
-extern template pi_status launch_decode_pitch<64>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
-extern template pi_status launch_decode_pitch<96>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
-extern template pi_status launch_decode_pitch<128>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
-extern template pi_status launch_decode_pitch<192>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
-extern template pi_status launch_decode_pitch<256>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int);
+extern template pi_status launch_decode_pitch<32>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int, int);
+extern template pi_status launch_decode_pitch<64>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int, int);
+extern template pi_status launch_decode_pitch<96>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int, int);
+extern template pi_status launch_decode_pitch<128>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int, int);
+extern template pi_status launch_decode_pitch<192>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int, int);
+extern template pi_status launch_decode_pitch<256>(pi_ctx*, int, int, int, const pi_kv8_attn_params&, dim3, int, int);
 
 }  // namespace pi_kv8

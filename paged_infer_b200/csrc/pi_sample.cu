@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   const int r = blockIdx.x / ranks;
   const int from = min((int)rank * p.per, p.n), count = min(p.per, p.n - from);
   const size_t base = (size_t)r * p.stride + from;
+  pi_grid_dependency_wait();
 
   // the slice, and the largest logit with the lowest index; NaN counts as minus infinity, -0 as 0
   unsigned long long best = 0;
@@ -356,18 +357,8 @@ extern "C" pi_status pi_sample(pi_ctx* ctx, const void* logits_dev, int dtype, s
     PI_CUDA(ctx, cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceFloats * (int)sizeof(float)));
     grant.of(ctx) = kSliceFloats * sizeof(float);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows * cluster);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
   pi_prof_scope prof(ctx, PI_PROF_OTHER);
-  PI_CUDA(ctx, cudaLaunchKernelEx(&cfg, sample_kernel, p));
+  PI_CUDA(ctx, pi_launch_chained(ctx, sample_kernel, dim3((unsigned)rows * cluster), dim3(kThreads), smem, cluster, p));
   PI_CHECK_LAUNCH(ctx);
   return PI_OK;
 }

@@ -9,7 +9,7 @@
 // the latency of a launch, of one load and of the scan.
 #include <algorithm>
 
-#include "pi_common.cuh"
+#include "pi_kv8.cuh"
 
 namespace {
 
@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const PlanParam
   const int B = p.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = p.a.block_size, wide = p.a.max_blocks;
   int *s_cu = s_plan, *s_free = s_cu + B + 1, *s_start = s_free + B;   // first row, first entry of the free list, start
   __shared__ Totals s_warp[kPlanWarps];
+  pi_grid_dependency_wait();
 
   // prefix sums: a run of sequences per thread, a scan of the runs' totals
   const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, B), b1 = min(b0 + per, B);
@@ -157,7 +158,8 @@ extern "C" pi_status pi_step_plan(pi_ctx* ctx, const pi_step_arrays* a, const in
   }
   const long long shares = std::max<long long>({1, ((long long)a->max_rows + kPlanThreads - 1) / kPlanThreads, ((long long)n_seqs + kPlanWarps - 1) / kPlanWarps});
   pi_prof_scope prof(ctx, PI_PROF_OTHER);
-  step_plan_kernel<<<(unsigned)std::min<long long>(shares, ctx->sm_count), kPlanThreads, smem, ctx->stream>>>({*a, start_dev, n_tokens_dev, free_dev, n_seqs, n_free});
+  const PlanParams p = {*a, start_dev, n_tokens_dev, free_dev, n_seqs, n_free};
+  PI_CUDA(ctx, pi_launch_chained(ctx, step_plan_kernel, dim3((unsigned)std::min<long long>(shares, ctx->sm_count)), dim3(kPlanThreads), smem, 1, p));
   PI_CHECK_LAUNCH(ctx);
   return PI_OK;
 }
