@@ -5,7 +5,7 @@
 // them.  Out of the kept tokens, in the order of their indices, comes the first whose running sum of w exceeds u times their sum.
 //
 // Every set above is a beginning of the order, so it is (threshold, number of tokens that equal it); neither a sort nor a list of
-// the kept tokens is needed.  The tokens that can matter (w above 2^-46, or min_p) are counted in 512 bins of equal width between
+// the kept tokens is needed.  The tokens that can matter (w above 2^-46, or min_p) are counted in 1024 bins of equal width between
 // the smallest and the largest of them.  Counts lead to the bin of the top_k-th token; counts times the weight in the middle of a
 // bin lead to the three bins that should hold the end of the nucleus, which the one pass that takes the weights of all kept tokens
 // confirms or moves.  Inside them the threshold is found digit by digit over the logits' ordered bit patterns, by exact sums.
@@ -15,8 +15,9 @@
 // and each of three 15-bit limbs of the tokens of a CTA room in 32, which is what histograms of weights add with the 32-bit atomics
 // of shared memory.
 //
-// A cluster of CTAs takes a row: each holds its slice of the logits in shared memory, so that they are read once, and reads the
-// others' histograms there.
+// A cluster of CTAs takes a row: each holds its slice of the logits in shared memory, so that they are read once.  A histogram is
+// made in each CTA's own memory; then every bin has a home in one of them, to which the others add theirs, and everybody reads all
+// bins from their homes.  (Reading all histograms of all eight CTAs instead cost twice as much as everything else together.)
 #include <float.h>
 
 #include <algorithm>
@@ -25,9 +26,10 @@
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = kThreads, kBinBits = 9, kMaxCluster = 8;   // a bin per thread
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2 * kThreads, kBinBits = 10, kMaxCluster = 8;   // two bins per thread
 constexpr int kWeightBits = 45, kLimb = 15;
 constexpr int kSliceFloats = 48 * 1024;   // logits that fit a CTA's shared memory beside the histograms
+constexpr int kTable = 32;                // floats that 16 doubles take
 
 struct SampleParams {
   const void* logits;
@@ -43,7 +45,8 @@ struct SampleParams {
 
 // What a CTA shows the others.
 struct Shown {
-  unsigned long long best;            // ordered logit << 32 | ~index
+  unsigned int most;                  // ordered logit
+  unsigned int at;                    // lowest index of the row's largest
   unsigned long long sums[2][3];      // of the kept weights: all, above the interval, in it (two buffers)
   unsigned long long weight;          // above the threshold
   unsigned int ties;
@@ -95,10 +98,10 @@ struct Row {
   int count;
   float most, scale;    // bins per unit of logit
   double rate;          // log2(e) / T
-  const double* roots;
   // 2^y for y = (v - most) rate <= 0: a sixteenth from the table, the rest g, |g| <= 1/32, by its series up to g^6 (the next term is below
   // 2^-51), as a multiple of 2^-45
   __device__ __forceinline__ unsigned long long weight(float v) const {
+    extern __shared__ __align__(16) float s_slice[];
     if (v == most) return 1ull << kWeightBits;
     const double y = ((double)v - (double)most) * rate;
     if (!(y > -60.0)) return 0;
@@ -111,7 +114,7 @@ struct Row {
     e = fma(e, g, 5.550410866482158e-2);
     e = fma(e, g, 2.402265069591007e-1);
     e = fma(e, g, 6.931471805599453e-1);
-    const double root = roots[k & 15];
+    const double root = reinterpret_cast<const double*>(s_slice)[k & 15];   // the table lies in front of the slice
     e = fma(e * g, root, root);
     const int n = (k >> 4) + kWeightBits;                          // times 2^n, n >= -15
     const double w = __hiloint2double(__double2hiint(e) + (n << 20), __double2loint(e)) + 4503599627370496.0;   // 2^52: rounds to a whole number
@@ -121,8 +124,7 @@ struct Row {
 };
 
 struct Shared {
-  uint32_t hist[2][3][kBins];
-  double roots[16];
+  uint32_t hist[3][kBins];             // of this CTA
   unsigned long long warp_a[kWarps], warp_sum[kWarps];
   unsigned long long warp_s[3][kWarps];
   float warp_f[kWarps];
@@ -153,49 +155,76 @@ __device__ __forceinline__ T scan(T v, T* s_warp, T& all) {
   return v;
 }
 
+// In dynamic shared memory: the table of roots, the cluster's totals of the bins that live here (three turns of kBins / CTAs), the slice.
+__device__ __forceinline__ unsigned long long* home_bins() {
+  extern __shared__ __align__(16) float s_slice[];
+  return reinterpret_cast<unsigned long long*>(s_slice + kTable);
+}
+
+// Two bins per thread, the ones of thread 0 first: the CTA's amounts in, the cluster's out.  A turn's buffer is cleared a turn ahead:
+// by then everybody has passed the barrier behind which nobody reads what it held two turns ago.
+__device__ __forceinline__ void exchange(unsigned long long* v, int& turn) {
+  const uint32_t tid = threadIdx.x, share = kBins / cluster_size(), home = 2 * tid / share;
+  unsigned long long *homes = home_bins(), *at = homes + turn % 3 * share + (2 * tid - home * share);
+  if (2 * tid < share) homes[(turn + 1) % 3 * share + 2 * tid] = homes[(turn + 1) % 3 * share + 2 * tid + 1] = 0;
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(home));
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (v[e]) asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(a + 8 * e), "l"(v[e]) : "memory");
+  cluster_sync();
+  asm volatile("ld.shared::cluster.v2.u64 {%0,%1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "r"(a) : "memory");
+  ++turn;
+}
+
 // The tokens of bins first .. last, ordered by their bit patterns k, lo <= k <= hi: the largest k for which `above` and the amounts (counts, or
 // weights) of tokens of at least k reach `want`; `above` becomes the amount above k.  By weight, tokens that equal `low` are left
 // out and `low_weight` stands for them.
 template <bool WEIGHT>
 __device__ uint32_t refine(const Row& row, Shared& s, int first, int last, uint32_t lo, uint32_t hi, uint32_t low, unsigned long long low_weight, unsigned long long want,
                            int& turn, unsigned long long& above) {
-  const int tid = threadIdx.x;
-  const uint32_t ranks = cluster_size();
+  const int tid = threadIdx.x, digit = kBins - 1 - 2 * tid;   // the largest first
   while (lo < hi) {
     const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
-    uint32_t(*h)[kBins] = s.hist[turn & 1];
-    ++turn;
 #pragma unroll
-    for (int i = 0; i < (WEIGHT ? 3 : 1); ++i) h[i][tid] = 0;
+    for (int i = 0; i < (WEIGHT ? 3 : 1); ++i) s.hist[i][tid] = s.hist[i][tid + kThreads] = 0;
     __syncthreads();
+    const float from = from_ordered(lo), to = from_ordered(hi);
+#pragma unroll 4
     for (int i = tid; i < row.count; i += kThreads) {
       const float x = row.x[i];
-      const uint32_t k = ordered(x);
-      if (k < lo || k > hi) continue;
-      const int b = row.bin(x);
-      if (b < first || b > last) continue;
-      const uint32_t digit = (k - lo) >> shift;
-      if (!WEIGHT) {
-        atomicAdd(&h[0][digit], 1u);
-      } else if (k != low) {
-        const unsigned long long w = row.weight(x);
-        atomicAdd(&h[0][digit], (uint32_t)w & 0x7fffu);
-        atomicAdd(&h[1][digit], (uint32_t)(w >> kLimb) & 0x7fffu);
-        atomicAdd(&h[2][digit], (uint32_t)(w >> 2 * kLimb));
+      if (x >= from && x <= to) {
+        const int b = row.bin(x);
+        const uint32_t k = ordered(x), d = (k - lo) >> shift;
+        if (b >= first && b <= last && k - lo <= hi - lo) {   // 0 passes for -0 above
+          if (!WEIGHT) {
+            atomicAdd(&s.hist[0][d], 1u);
+          } else if (k != low) {
+            const unsigned long long w = row.weight(x);
+            atomicAdd(&s.hist[0][d], (uint32_t)w & 0x7fffu);
+            atomicAdd(&s.hist[1][d], (uint32_t)(w >> kLimb) & 0x7fffu);
+            atomicAdd(&s.hist[2][d], (uint32_t)(w >> 2 * kLimb));
+          }
+        }
       }
     }
-    cluster_sync();
-    const int digit = kBins - 1 - tid;   // the largest first
-    unsigned long long v = 0, all;
-    for (uint32_t r = 0; r < ranks; ++r) {
-      v += peer(&h[0][digit], r);
-      if (WEIGHT) v += ((unsigned long long)peer(&h[1][digit], r) << kLimb) + ((unsigned long long)peer(&h[2][digit], r) << 2 * kLimb);
+    __syncthreads();
+    unsigned long long v[2], all;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      v[e] = s.hist[0][digit - e];
+      if (WEIGHT) v[e] += ((unsigned long long)s.hist[1][digit - e] << kLimb) + ((unsigned long long)s.hist[2][digit - e] << 2 * kLimb);
     }
-    if (WEIGHT && digit == 0 && lo == low) v += low_weight;
-    const unsigned long long upto = above + scan(v, s.warp_a, all);
-    if (upto >= want && upto - v < want) {
-      s.bin = digit;
-      s.above = upto - v;
+    exchange(v, turn);
+    if (WEIGHT && tid == kThreads - 1 && lo == low) v[1] += low_weight;
+    unsigned long long upto = above + scan(v[0] + v[1], s.warp_a, all) - v[1];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (upto >= want && upto - v[e] < want) {
+        s.bin = digit - e;
+        s.above = upto - v[e];
+      }
+      upto += v[1];
     }
     __syncthreads();
     above = s.above;
@@ -214,16 +243,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int r = blockIdx.x / ranks;
   const int from = min((int)rank * p.per, p.n), count = min(p.per, p.n - from);
   const size_t base = (size_t)r * p.stride + from;
-  if (tid < 16) s.roots[tid] = kRoots[tid];
+  float* const slice = s_slice + kTable + 6 * kBins / ranks;
+  if (tid < 16) reinterpret_cast<double*>(s_slice)[tid] = kRoots[tid];
   pi_grid_dependency_wait();
 
-  // the slice, and the largest logit with the lowest index; NaN counts as minus infinity, -0 as 0
-  unsigned long long best = 0;
-  auto take = [&](int i, float x) {
-    x = x == x ? x + 0.f : -INFINITY;
-    s_slice[i] = x;
-    best = max(best, (unsigned long long)ordered(x) << 32 | (uint32_t)~(from + i));
-  };
+  // the slice, and the largest logit; NaN counts as minus infinity, -0 as 0
+  float best = -INFINITY;
   if (p.wide) {
     const int whole = count & ~3;
 #pragma unroll 4
@@ -231,30 +256,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       float x[4];
       pi_load4_as_f32(x, p.logits, base + i, p.dtype, 4, true);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) take(i + e, x[e]);
+      for (int e = 0; e < 4; ++e) {
+        x[e] = fmaxf(x[e], -INFINITY) + 0.f;
+        best = fmaxf(best, x[e]);
+      }
+      *reinterpret_cast<float4*>(slice + i) = make_float4(x[0], x[1], x[2], x[3]);
     }
-    if (whole + tid < count) take(whole + tid, pi_load_as_f32(p.logits, base + whole + tid, p.dtype));
+    if (whole + tid < count) best = fmaxf(best, slice[whole + tid] = fmaxf(pi_load_as_f32(p.logits, base + whole + tid, p.dtype), -INFINITY) + 0.f);
   } else {
 #pragma unroll 4
-    for (int i = tid; i < count; i += kThreads) take(i, pi_load_as_f32(p.logits, base + i, p.dtype));
+    for (int i = tid; i < count; i += kThreads) best = fmaxf(best, slice[i] = fmaxf(pi_load_as_f32(p.logits, base + i, p.dtype), -INFINITY) + 0.f);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) s.warp_a[warp] = best;
-  s.hist[0][0][tid] = 0;
+  best = pi_warp_max(best);
+  if (lane == 0) s.warp_f[warp] = best;
+  s.hist[0][tid] = s.hist[0][tid + kThreads] = 0;
+  if (2 * tid < kBins / ranks) home_bins()[2 * tid] = home_bins()[2 * tid + 1] = 0;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) best = max(best, s.warp_a[w]);
-    s.shown.best = best;
+    for (int w = 1; w < kWarps; ++w) best = fmaxf(best, s.warp_f[w]);
+    s.shown.most = ordered(best);
+    s.shown.at = 0x7fffffff;
   }
   cluster_sync();
-  best = 0;
-  for (uint32_t k = 0; k < ranks; ++k) best = max(best, peer(&s.shown.best, k));
-  const uint32_t high = (uint32_t)(best >> 32);
+  const uint32_t high = __reduce_max_sync(0xffffffffu, lane < ranks ? peer(&s.shown.most, lane) : 0);
   const float most = from_ordered(high), temperature = p.temperature[r];
-  if (!(temperature > 0.f) || most == -INFINITY) {   // the largest; a row without any
+  if (!(temperature > 0.f) || most == -INFINITY) {   // the largest, the lowest index of equal ones; a row without any
+    for (int i = tid; i < count; i += kThreads)
+      if (slice[i] == most) {
+        atomicMin(&s.shown.at, (unsigned int)(from + i));
+        break;
+      }
+    cluster_sync();
     if (rank == 0 && tid == 0) {
-      p.ids[r] = most == -INFINITY ? -1 : (int32_t)~(uint32_t)best;
+      unsigned int at = 0x7fffffff;
+      for (uint32_t q = 0; q < ranks; ++q) at = min(at, peer(&s.shown.at, q));
+      p.ids[r] = most == -INFINITY ? -1 : (int32_t)at;
       if (p.probs) p.probs[r] = most == -INFINITY ? 0.f : 1.f;
     }
     cluster_sync();
@@ -265,23 +301,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const float min_p = p.min_p[r];
   if (min_p > 0.f) exact_bound = max(exact_bound, (double)most + (double)temperature * log(min((double)min_p, 1.0)));
   const float bound = most == INFINITY ? INFINITY : max(__double2float_ru(exact_bound), -FLT_MAX);
-  const Row row = {s_slice, count, most, (float)kBins / (most - bound), 1.4426950408889634 / (double)temperature, s.roots};
+  const Row row = {slice, count, most, (float)kBins / (most - bound), 1.4426950408889634 / (double)temperature};
 
   const int k = p.top_k[r];
   const float top_p = p.top_p[r];
   const bool by_count = k > 0 && k < p.n, by_weight = top_p < 1.f;
-  uint32_t thr = ordered(bound) - 1;           // kept: above thr, and the first `ties` that equal it
+  // kept: above thr, and the first `ties` that equal it; the number below 0 is not -0, which equals it
+  uint32_t thr = ordered(bound) - (bound == 0.f ? 2 : 1);
   unsigned long long ties = 0, above = 0;
-  int turn = 1, first = 0;                     // bins in front of `first`: their weights are in warp_sum already
+  int turn = 0, first = 0;                     // bins in front of `first`: their weights are in warp_sum already
   unsigned long long interval_above = 0;
   if (tid < kWarps) s.warp_sum[tid] = 0;
+  float sure = INFINITY;                       // logits above it lie in those bins
   if (by_count || by_weight) {
-    for (int i = tid; i < count; i += kThreads)
-      if (s_slice[i] >= bound) atomicAdd(&s.hist[0][0][row.bin(s_slice[i])], 1u);
-    cluster_sync();
-    unsigned int here = 0, all;
-    for (uint32_t q = 0; q < ranks; ++q) here += peer(&s.hist[0][0][tid], q);
-    unsigned int upto = scan(here, s.warp_b, all);
+#pragma unroll 4
+    for (int i = tid; i < count; i += kThreads) {
+      const float x = slice[i];
+      if (x >= bound) atomicAdd(&s.hist[0][row.bin(x)], 1u);
+    }
+    __syncthreads();
+    unsigned long long v[2] = {s.hist[0][2 * tid], s.hist[0][2 * tid + 1]};
+    exchange(v, turn);
+    unsigned int here[2] = {(unsigned int)v[0], (unsigned int)v[1]}, upto[2], all;
+    upto[1] = scan(here[0] + here[1], s.warp_b, all);
+    upto[0] = upto[1] - here[1];
     // logits at the edges of a bin, a little outside
     const float step = (most - bound) / (float)kBins, slack = fmaxf(fabsf(most), fabsf(bound)) * 1e-6f;
     auto upper = [&](int b) {
@@ -294,39 +337,52 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     };
     int last_bin = kBins - 1;
     if (by_count && all > (unsigned int)k) {
-      if (upto >= (unsigned int)k && upto - here < (unsigned int)k) {
-        s.bin = tid;
-        s.above = upto - here;
-      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (upto[e] >= (unsigned int)k && upto[e] - here[e] < (unsigned int)k) {
+          s.bin = 2 * tid + e;
+          s.above = upto[e] - here[e];
+        }
       __syncthreads();
       last_bin = s.bin;
       above = s.above;
       __syncthreads();
       thr = refine<false>(row, s, last_bin, last_bin, lower(last_bin), upper(last_bin), 0, 0, (unsigned long long)k, turn, above);
       ties = (unsigned long long)k - above;
-      const unsigned int before = min(upto - here, (unsigned int)k);
-      here = min(upto, (unsigned int)k) - before;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) here[e] = min(upto[e], (unsigned int)k) - min(upto[e] - here[e], (unsigned int)k);
     }
     if (by_weight) {
       // where the nucleus should end
       float sum;
-      const float hint = (float)here * exp2f(-((float)tid + 0.5f) * step * (float)row.rate), hints = scan(hint, s.warp_f, sum);
+      float hint[2], hints[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) hint[e] = (float)here[e] * exp2f(-((float)(2 * tid + e) + 0.5f) * step * (float)row.rate);
+      hints[1] = scan(hint[0] + hint[1], s.warp_f, sum);
+      hints[0] = hints[1] - hint[1];
       const unsigned long long low_weight = ties * row.weight(from_ordered(thr));
       const int low_bin = ties ? row.bin(from_ordered(thr)) : kBins;
       float goal = fmaxf(top_p, 0.f) * sum;   // identical in all CTAs, as all that steers them is
       unsigned long long want = 0, inside = 0;
       int last = 0;
       for (int round = 0;; ++round) {
-        const int middle = min(__syncthreads_count(hints < goal), last_bin);
+        if (tid == 0) s.bin = 0;
+        __syncthreads();
+        const int under = __popc(__ballot_sync(0xffffffffu, hints[0] < goal)) + __popc(__ballot_sync(0xffffffffu, hints[1] < goal));
+        if (lane == 0) atomicAdd(&s.bin, under);
+        __syncthreads();
+        const int middle = min(s.bin, last_bin);
         first = max(0, middle - 1);
         last = min(last_bin, middle + 1);
         if (round >= 6) first = 0, last = last_bin;   // whatever the estimate says
         // exact sums: a run of the slice per warp, so that they serve the draw as well
         const int run = ((count + kWarps * 32 - 1) / (kWarps * 32)) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
         unsigned long long in_front = 0, in = 0, behind = 0;
+        const float least = from_ordered(thr);
+#pragma unroll 2
         for (int i = i0 + lane; i < i1; i += 32) {
-          const float x = s_slice[i];
-          if (ordered(x) > thr) {
+          const float x = slice[i];
+          if (x > least) {
             const int b = row.bin(x);
             const unsigned long long w = row.weight(x);
             if (b < first) in_front += w;
@@ -351,21 +407,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
         cluster_sync();
         unsigned long long t[3] = {low_weight, low_bin < first ? low_weight : 0, low_bin >= first && low_bin <= last ? low_weight : 0};
-        for (uint32_t q = 0; q < ranks; ++q)
 #pragma unroll
-          for (int e = 0; e < 3; ++e) t[e] += peer(&s.shown.sums[round & 1][e], q);
+        for (int e = 0; e < 3; ++e) t[e] += warp_sum(lane < ranks ? peer(&s.shown.sums[round & 1][e], lane) : 0);
         want = min(max(1ull, (unsigned long long)ceil((double)fmaxf(top_p, 0.f) * (double)t[0])), t[0]);
         interval_above = t[1];
         inside = t[2];
         if (interval_above < want && want <= interval_above + inside) break;
         // the estimate again, from the exact sum in front of the interval
-        if (tid == first) s.warp_f[0] = hints - hint;
+        if (tid == first / 2) s.warp_f[0] = hints[first & 1] - hint[first & 1];
         __syncthreads();
         goal = s.warp_f[0] + ((float)((double)want - (double)interval_above)) * (1.f / (float)(1ull << kWeightBits));
         if (want <= interval_above) goal = fminf(goal, s.warp_f[0] * 0.9999999f);
         __syncthreads();
       }
       above = interval_above;
+      if (first > 0) sure = from_ordered(upper(first));
       const uint32_t low = thr;
       thr = refine<true>(row, s, first, last, max(low, last == last_bin ? low : lower(last)), upper(first), low, low_weight, want, turn, above);
       const unsigned long long w = row.weight(from_ordered(thr));
@@ -377,10 +433,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int run = ((count + kWarps * 32 - 1) / (kWarps * 32)) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
   unsigned long long sum = 0;
   unsigned int same = 0;
+  const float least = from_ordered(thr);
+#pragma unroll 4
   for (int i = i0 + lane; i < i1; i += 32) {
-    const uint32_t key = ordered(s_slice[i]);
-    if (key > thr && (first == 0 || row.bin(s_slice[i]) >= first)) sum += row.weight(s_slice[i]);
-    same += key == thr;
+    const float x = slice[i];
+    if (x > least && !(x > sure) && row.bin(x) >= first) sum += row.weight(x);
+    same += x == least;
   }
   sum = warp_sum(sum);
   same = __reduce_add_sync(0xffffffffu, same);
@@ -402,14 +460,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
   cluster_sync();
   const unsigned long long w_thr = row.weight(from_ordered(thr));
-  unsigned long long total = 0, ahead = 0, used = 0, used_here = 0;
-  for (uint32_t q = 0; q < ranks; ++q) {
-    const unsigned long long equal = min((unsigned long long)peer(&s.shown.ties, q), ties - used), v = peer(&s.shown.weight, q) + equal * w_thr;
-    if (q < rank) ahead += v;
-    if (q == rank) used_here = used;
-    used += equal;
-    total += v;
+  // lane q looks at CTA q: how many of its equal tokens are kept, and what it holds
+  unsigned int equals = lane < ranks ? peer(&s.shown.ties, lane) : 0, upto_equals = equals;
+#pragma unroll
+  for (int o = 1; o < kMaxCluster; o <<= 1) {
+    const unsigned int t = __shfl_up_sync(0xffffffffu, upto_equals, o);
+    if (lane >= o) upto_equals += t;
   }
+  const unsigned long long used = min((unsigned long long)(upto_equals - equals), ties), held = (lane < ranks ? peer(&s.shown.weight, lane) : 0) + (min((unsigned long long)upto_equals, ties) - used) * w_thr;
+  const unsigned long long total = warp_sum(lane < ranks ? held : 0), ahead = warp_sum(lane < rank ? held : 0), used_here = __shfl_sync(0xffffffffu, used, rank);
   const float u = p.u[r];
   unsigned long long goal = u > 0.f ? (unsigned long long)floor((double)u * (double)total) : 0;
   goal = min(goal, total - 1);
@@ -423,11 +482,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const unsigned long long here = s.warp_a[warp] + min((unsigned long long)s.warp_b[warp], ties - taken) * w_thr;
   if (goal >= mine && goal < mine + here) {
     for (int i = i0 + lane; i - lane < i1; i += 32) {
-      const uint32_t key = i < i1 ? ordered(s_slice[i]) : 0;
-      const unsigned equal = __ballot_sync(0xffffffffu, i < i1 && key == thr);
+      const float x = i < i1 ? slice[i] : -INFINITY;
+      const unsigned equal = __ballot_sync(0xffffffffu, i < i1 && x == least);
       unsigned long long w = 0;
-      if (i < i1 && key > thr) w = row.weight(s_slice[i]);
-      if (i < i1 && key == thr && taken + __popc(equal & ((1u << lane) - 1)) < ties) w = w_thr;
+      if (x > least) w = row.weight(x);
+      if (i < i1 && x == least && taken + __popc(equal & ((1u << lane) - 1)) < ties) w = w_thr;
       taken += __popc(equal);
       unsigned long long upto = w;
 #pragma unroll
@@ -468,11 +527,12 @@ extern "C" pi_status pi_sample(pi_ctx* ctx, const void* logits_dev, int dtype, s
   const size_t size = dtype == PI_F32 ? 4 : 2;
   const bool wide = (uintptr_t)logits_dev % (4 * size) == 0 && (rows == 1 || row_stride % 4 == 0);
   SampleParams p = {logits_dev, dtype, row_stride, n, per, wide, temperature_dev, top_p_dev, min_p_dev, u_dev, top_k_dev, ids_dev, probs_dev_or_null};
-  const size_t smem = (size_t)p.per * sizeof(float);
+  const size_t smem = (size_t)(kTable + 6 * kBins / cluster + p.per) * sizeof(float);
+  constexpr int kMostShared = (kTable + 6 * kBins / kMaxCluster + kSliceFloats) * (int)sizeof(float);   // of the longest row; smaller clusters have shorter slices
   static pi_smem_grant grant;
   if (smem > grant.of(ctx)) {
-    PI_CUDA(ctx, cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceFloats * (int)sizeof(float)));
-    grant.of(ctx) = kSliceFloats * sizeof(float);
+    PI_CUDA(ctx, cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+    grant.of(ctx) = kMostShared;
   }
   pi_prof_scope prof(ctx, PI_PROF_OTHER);
   PI_CUDA(ctx, pi_launch_chained(ctx, sample_kernel, dim3((unsigned)rows * cluster), dim3(kThreads), smem, cluster, p));
