@@ -590,6 +590,7 @@ __device__ __forceinline__ void pi_grid_dependency_wait() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+__device__ __forceinline__ void pi_grid_dependency_wait_only() { asm volatile("griddepcontrol.wait;" ::: "memory"); }   // and release later
 __device__ __forceinline__ void pi_grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // The other order: nothing queued behind this grid starts before the grid ahead of it has completed.  One such kernel
 // in a chain is a fence for early reads: whatever ran before it is complete in the eyes of EVERY later kernel, even in

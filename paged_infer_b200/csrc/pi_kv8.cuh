@@ -53,8 +53,12 @@ struct pi_kv8_attn_params {
   int max_blocks, n_seqs, n_rows;
   int window;                    // <= 0: none
   float scale2;                  // of the scores, times log2(e)
+  int max_cols;                  // decode: sequences with more columns are another kernel's
 };
-pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn_params& p, int max_seq_rows, int max_context);
+// Sequences of at most max_cols columns (rows times group), and those of more than min_cols.
+pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn_params& p, int max_seq_rows, int max_context, int max_cols);
+bool pi_kv8_prefill_takes(const pi_kv8_pool* pool, int group);
+pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_kv8_attn_params& p, int min_cols, int max_context);
 
 // A launch on the context's stream that may begin while the kernel ahead of it ends (every kernel waits for that one before it touches
 // memory), in clusters of `cluster` CTAs along x.

@@ -3,7 +3,12 @@
 
 using namespace pi_kv8;
 
-pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn_params& p, int max_seq_rows, int max_context) {
+namespace {
+constexpr int kFewColumns = 16;
+}
+
+pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn_params& p, int max_seq_rows, int max_context, int max_cols) {
+  p.max_cols = max_cols;
   // eight columns a product; sixteen where a sequence brings more, so that its codes are widened half as often
   const long long cols = (long long)max_seq_rows * p.group;
   const int nt = cols <= 8 ? 1 : 2, planes = p.dtype == PI_F32 ? 2 : 1;
@@ -83,5 +88,11 @@ extern "C" pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int 
   p.window = window;
   p.scale2 = scale * 1.4426950408889634f;
   pi_prof_scope prof(ctx, PI_PROF_ATTENTION);
-  return pi_launch_kv8_decode(ctx, pool, p, std::min(max_seq_rows, n_rows), max_context);
+  max_seq_rows = std::min(max_seq_rows, n_rows);
+  // Sequences of up to 16 columns (the widest product of the one kernel) beside longer portions: each kernel takes its own, whatever the
+  // lengths on the device are.  A sequence alone is a portion.
+  if ((long long)max_seq_rows * p.group <= kFewColumns || !pi_kv8_prefill_takes(pool, p.group)) return pi_launch_kv8_decode(ctx, pool, p, max_seq_rows, max_context, 0x7fffffff);
+  if (n_seqs == 1) return pi_launch_kv8_prefill(ctx, pool, p, 0, max_context);
+  if (p.group <= kFewColumns) PI_TRY(pi_launch_kv8_decode(ctx, pool, p, kFewColumns / p.group, max_context, kFewColumns));
+  return pi_launch_kv8_prefill(ctx, pool, p, p.group <= kFewColumns ? kFewColumns : 0, max_context);
 }

@@ -25,16 +25,11 @@
 
 #include <algorithm>
 
-#include "pi_kv8.cuh"
-#include "pi_mma.cuh"
+#include "pi_kv8_widen.cuh"
 
 namespace pi_kv8 {
 
 constexpr int kMaxSplit = 16, kMaxWarps = 8;   // CTAs of a cluster, warps of a CTA
-// Weights are stored times 2^7 relative to a running maximum that may lag 2^8 behind: at most 2^15, below the largest f16, and
-// precise down to 2^-21 (one plane: of the largest).  The maximum is only taken across lanes when a score exceeds it by more.
-constexpr float kTopWeight = 7.f, kLag = 8.f;
-
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -52,11 +47,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // of an 8 x 8 ti
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Codes are read once.
 template <int BYTES>
 __device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* from) {
@@ -70,41 +60,7 @@ __device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* from) {
     to[0] = __ldcs(reinterpret_cast<const uint32_t*>(from));
   }
 }
-// How much a partial result (maximum, sum) counts beside the maximum of all: one that saw nothing does not, one that is not a
-// number makes the whole one.
-__device__ __forceinline__ float join_factor(float top, float sum, float all) {
-  if (sum != sum) return sum;
-  return top == -INFINITY ? 0.f : exp2_fast(top - all);
-}
-// Two codes as f16: bytes 0 and 1, or 2 and 3, of a word.  int8 (its sign bit flipped): 1024 + (code + 128) in the mantissa, less 1152
-// unless that stays in.
-template <int KIND, bool BIASED>
-__device__ __forceinline__ uint32_t widen(uint32_t w, bool high) {
-  if (KIND == PI_INT8) {
-    const uint32_t h = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
-    if (BIASED) return h;
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(high ? w >> 16 : w)));
-  return h;
-}
-template <int KIND>
-__device__ __forceinline__ uint32_t unsign(uint32_t w) {
-  return KIND == PI_INT8 ? w ^ 0x80808080u : w;
-}
 constexpr float kBias = 1152.f;
-
-// f16 pair of two values and the pair of what is left.
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return pack_f16(a - f.x, b - f.y);
-}
 
 template <int PITCH>
 struct Geometry {
@@ -114,22 +70,6 @@ struct Geometry {
   // V: PITCH / 8 neighbouring channels of a token, in pieces of VB bytes
   static constexpr int VB = PITCH % 128 == 0 ? 16 : PITCH % 64 == 0 ? 8 : 4, vpieces = PITCH / 8 / VB;
 };
-
-__device__ __forceinline__ uint32_t peer_addr(const void* mine, uint32_t rank) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(pi_mma::smem_addr(mine)), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ float2 peer2(const float2* mine, uint32_t rank) {   // the same variable of another CTA of the cluster
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_addr(mine, rank)) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 peer4(const float* mine, uint32_t rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_addr(mine, rank)) : "memory");
-  return v;
-}
 
 // Tiles that a warp works on at a time, and CTAs of eight warps that an SM has registers for: sixteen warps hide the chain from load
 // to product to exponential to product better than eight with longer steps (24 with 80 registers spill); wide heads and two groups
@@ -171,7 +111,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
   const int kvh = blockIdx.x / splits, seq = blockIdx.y, bs = p.block_size;
   pi_grid_dependency_wait();
   const int row_begin = max(0, min(p.cu_rows[seq], p.n_rows)), row_end = min(p.cu_rows[seq + 1], p.n_rows);
-  const int ncols = (row_end - row_begin) * p.group;
+  const int ncols = (row_end - row_begin) * p.group > p.max_cols ? 0 : (row_end - row_begin) * p.group;
   const int last_token = (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1;
   const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
   // one tile of columns as the grid is cut; the loop is for sequences that bring more rows than the call said

@@ -1,0 +1,634 @@
+// Paged attention over the 8-bit cache for sequences that bring many rows (portions of prompts), on tcgen05: accumulators and the A
+// operands in tensor memory, B operands in shared memory.  Head sizes that are stored in 64 or 128 bytes.
+//
+// A CTA owns 128 (row, query head) pairs of one sequence and KV head, one per TMEM lane, and walks the positions that they see in tiles
+// of 64 columns: four times 16 tokens, each of one block and with one pair of scales.  Codes are widened to f16, which holds them
+// exactly; queries (brought to [-1, 1] by a power of two per row) and weights are f16 too, in two planes (22 bits) for f32 tensors:
+//     scores  S = Q K^T        A = Q (written once),  B = codes of K, [token][channel]
+//     output  O = P V          A = P,                 B = codes of V transposed, [channel][token]
+// A row's thread multiplies the K scale in as it reads its scores, and weighs exp(score) by V scale / r, r a power of two above the
+// V scales that the row sees in the tile, so that P stays in f16's range whatever the scales are; the product of a tile is read
+// back, multiplied by r and added to the row's f32 output in registers.  The running maximum may lag 2^8 behind, so that the output
+// is hardly ever rescaled.
+//
+// Warps 0-3: a thread per row, with registers that the others give up.  Warps 4-7 and 8-11: the even and the odd tiles' codes, one of
+// theirs ahead in registers, then widened into shared memory (V by byte permutes of eight tokens at a time).  Warp 12: issues the
+// products (13-15 are there because registers are dealt to four warps at a time); the scores of tile j + 1 run while the rows work
+// on tile j.
+// Hand-offs go through mbarriers; every wait is bounded and raises the context's error word instead of hanging.  Where there are few
+// tiles of rows, a cluster shares the positions of one and joins its CTAs' outputs through shared memory.
+//
+// Bound: the rows' threads.  64 columns cost a row's thread 64 exponentials, of which an SM makes 16 a clock: 512 clocks, as long as
+// both products of a head of 128 channels; around them come a multiplication, a maximum, an addition and half a conversion each, and
+// reading back the tile's output.
+#include <math.h>
+
+#include <algorithm>
+
+#include "pi_kv8_widen.cuh"
+
+namespace {
+
+using namespace pi_kv8;
+
+constexpr int kRowsP = 128, kTileP = 64, kThreadsP = 16 * 32, kStagesP = 4;
+constexpr uint32_t kSpinP = 1u << 20, kNap = 256;   // polls, and the nanoseconds that each may sleep
+
+struct PrefillParams {
+  pi_kv8_attn_params a;
+  int rows_per_tile, min_cols;   // rows of a tile; sequences with fewer columns are another kernel's
+  int* err_flag;
+};
+
+// 16 tokens of a tile: first position, how many are there (0: not mapped), scale of K, scale of V as 2^v_exp 2^v_log, v_log in [0, 1).
+struct Group {
+  int base, valid;
+  float k_scale;
+  int v_exp;
+  float v_log;
+};
+constexpr int kNoScale = -100000;   // v_exp of a zero scale
+
+__device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t spin = 0; spin < kSpinP; ++spin) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity), "r"(kNap) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int lane) {
+  int ok = 1;
+  if (lane == 0) ok = (!*abort_flag && bar_wait(bar, parity)) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+// K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc),
+               "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void t_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void t_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]));
+}
+__device__ __forceinline__ void t_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void t_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int HD, int PLANES>
+struct Prefill {
+  static constexpr int side = kTileP * HD * 2, stage = 2 * side;   // bytes of a tile's K, and as many of V
+  static constexpr int line = HD + 4;                              // floats of a row where the CTAs of a cluster meet
+  static constexpr int rings = kStagesP * stage, meet = kRowsP * line * 4 + kRowsP * 8;
+  static constexpr int body = rings > meet ? rings : meet;
+  // at least 120 KB: two of these CTAs, each of which takes all of tensor memory, never share an SM
+  static constexpr int smem = (body > 119 * 1024 ? body : 119 * 1024) + 1024;
+  // tensor memory: two buffers of scores, the planes of P, the tile's output, the planes of Q
+  static constexpr uint32_t col_s = 0, col_p = 128, col_o = 192, col_q = 320;
+};
+
+template <int KIND, int HD, int PLANES>
+__global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const PrefillParams pp) {
+  using L = Prefill<HD, PLANES>;
+  const pi_kv8_attn_params& p = pp.a;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) unsigned long long bars[2 * kStagesP + 5];
+  __shared__ Group s_group[kStagesP][4];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+  __shared__ int s_lo, s_hi, s_seq, s_first;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = p.block_size, G = p.group;
+  uint32_t split, splits;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const int kvh = blockIdx.x / splits;
+  const uint32_t kv_full0 = s_u32(&bars[0]), kv_free0 = s_u32(&bars[kStagesP]), s_full0 = s_u32(&bars[2 * kStagesP]), p_full = s_u32(&bars[2 * kStagesP + 2]),
+                 o_full = s_u32(&bars[2 * kStagesP + 3]), o_free = s_u32(&bars[2 * kStagesP + 4]);
+  pi_grid_dependency_wait_only();
+
+  // the tile of rows: sequences' tiles are numbered through
+  if (warp == 0) {
+    int ahead = 0, seq = -1, first = 0;
+    for (int b0 = 0; b0 < p.n_seqs && seq < 0; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0, begin = 0;
+      if (b < p.n_seqs) {
+        begin = max(0, min(p.cu_rows[b], p.n_rows));
+        n = max(0, min(p.cu_rows[b + 1], p.n_rows) - begin);
+      }
+      const int tiles = n * G > pp.min_cols ? (n + pp.rows_per_tile - 1) / pp.rows_per_tile : 0;
+      int upto = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += t;
+      }
+      const int y = (int)blockIdx.y - ahead;
+      const unsigned hit = __ballot_sync(0xffffffffu, y < upto && y >= upto - tiles);
+      if (hit) {
+        const int at = __ffs(hit) - 1;
+        seq = b0 + at;
+        // a sequence's last rows see most: they come first
+        first = __shfl_sync(0xffffffffu, begin + (upto - 1 - y) * pp.rows_per_tile, at);
+      }
+      ahead += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) {
+      s_seq = seq;
+      s_first = first;
+      s_lo = 0x7fffffff;
+      s_hi = -1;
+      s_abort = 0;
+      for (int i = 0; i < kStagesP; ++i) {
+        bar_init(kv_full0 + 8 * i, 4);   // one arrival per converter warp
+        bar_init(kv_free0 + 8 * i, 1);   // tcgen05.commit
+      }
+      for (int i = 0; i < 2; ++i) bar_init(s_full0 + 8 * i, 1);
+      bar_init(p_full, 4);               // one arrival per row warp
+      bar_init(o_full, 1);
+      bar_init(o_free, 4);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+  }
+  __syncthreads();
+  const int seq = s_seq;
+  if (seq < 0) return;   // the whole cluster: fewer tiles than the grid allows for
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&s_tmem)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // this thread's row (warps 0-3)
+  const int row_end = min(p.cu_rows[seq + 1], p.n_rows), m = tid, local = p.by_group(m), head = m - local * G;
+  const bool live = warp < 4 && local < pp.rows_per_tile && s_first + local < row_end;
+  int pos = -1, from = 0;
+  if (live) {
+    pos = p.row_pos[s_first + local];
+    from = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+    if (pos >= 0) {
+      atomicMin(&s_lo, from);
+      atomicMax(&s_hi, pos);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  // the dependent grid is released only now that this CTA holds its tensor memory (a dependent CTA that took the SM's columns first
+  // would keep them until this grid completes)
+  pi_grid_launch_dependents();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = s_tmem, smem_base = s_u32(smem), lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  const int lo_all = s_lo, hi_all = min(s_hi, (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1);
+  const int per_block = (bs + 15) >> 4, first_block = hi_all < lo_all ? 0 : p.by_block(lo_all);
+  const int groups = hi_all < lo_all ? 0 : (p.by_block(hi_all) - first_block + 1) * per_block, tiles_all = (groups + 3) >> 2;
+  // this CTA's share of the positions: every splits-th tile
+  const int ntiles = tiles_all > (int)split ? (tiles_all - (int)split + (int)splits - 1) / (int)splits : 0;
+  const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
+
+  float factor = 0.f;
+  if (warp < 4) {
+    // the row's query: two readings, the largest channel first
+    const size_t at = live ? (size_t)(s_first + local) * p.q_stride + (size_t)(kvh * G + head) * p.head_dim : 0;
+    float most = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 4) {
+      float x[4];
+      pi_load4_as_f32(x, p.q, at + d, p.dtype, live ? p.head_dim - d : 0, p.q_wide);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) most = fmaxf(most, fabsf(x[b]));
+    }
+    const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);   // both powers stay normal
+    const float shrink = __uint_as_float((253u - e) << 23);
+    factor = __uint_as_float((e + 1) << 23) * p.scale2;
+#pragma unroll 2
+    for (int d = 0; d < HD; d += 16) {
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[4];
+        pi_load4_as_f32(x, p.q, at + d + 4 * i, p.dtype, live ? p.head_dim - d - 4 * i : 0, p.q_wide);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] *= shrink;
+        hi[2 * i] = pack_f16(x[0], x[1]);
+        hi[2 * i + 1] = pack_f16(x[2], x[3]);
+        if constexpr (PLANES == 2) {
+          lo[2 * i] = pack_rest(x[0], x[1], hi[2 * i]);
+          lo[2 * i + 1] = pack_rest(x[2], x[3], hi[2 * i + 1]);
+        }
+      }
+      __syncwarp();
+      t_st8(lane_addr + L::col_q + d / 2, hi);
+      if constexpr (PLANES == 2) t_st8(lane_addr + L::col_q + HD / 2 + d / 2, lo);
+    }
+    t_wait_st();
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  auto fail = [&](int code) {
+    if (!s_abort) {
+      s_abort = 1;
+      if (pp.err_flag) atomicExch(pp.err_flag, code);
+    }
+  };
+
+  float* s_out = reinterpret_cast<float*>(smem);   // where the CTAs of a cluster meet: outputs relative to their own maxima
+  float2* s_stat = reinterpret_cast<float2*>(s_out + kRowsP * L::line);
+  auto store = [&](int row_local, int h, int d, float4 v, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l, y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    if (d < p.head_dim)
+      pi_store4_f32_as(y, p.out, (size_t)(s_first + row_local) * p.out_stride + (size_t)(kvh * G + h) * p.head_dim + d, p.dtype, p.head_dim - d, p.out_wide);
+  };
+  // of the 512 registers that four warps of a lane's number have at launch, one of each group: 240 for a row, 96 for each group of
+  // converters, 80 for the rest
+  if (warp < 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
+    float acc[HD], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD; ++i) acc[i] = 0.f;
+    // ---- a thread per row ---------------------------------------------------------------------------------------------------
+    float fold_keep = 1.f, fold_unit = 0.f;   // of the tile before: what became of the output so far, and its r
+    bool alive = true;
+    const int to = min(pos, hi_all);
+    auto fold = [&](int j) -> bool {   // the product of tile j into the output
+      if (!warp_wait(o_full, j & 1, &s_abort, lane)) {
+        if (lane == 0) fail(22);
+        return false;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool shrunk = __any_sync(0xffffffffu, fold_keep != 1.f);
+#pragma unroll
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        t_ld16(lane_addr + L::col_o + c, o);
+        t_ld16(lane_addr + L::col_o + c + 16, o + 16);
+        t_wait_ld();
+        if (shrunk) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c + i] *= fold_keep;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(fold_unit, __uint_as_float(o[i]), acc[c + i]);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(o_free);
+      return true;
+    };
+    for (int j = 0; j < ntiles; ++j) {
+      const int buf = j & 1;
+      // the scores, and for the groups' scales what the converters released with the codes (this phase cannot pass before P is handed over)
+      if (!warp_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort, lane) || !warp_wait(kv_full0 + 8 * (j % kStagesP), (j / kStagesP) & 1, &s_abort, lane)) {
+        if (lane == 0) fail(21);
+        alive = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const Group* group = s_group[j % kStagesP];
+      const uint32_t s_col = lane_addr + L::col_s + buf * 64;
+      // what the row sees of each group: its columns first .. last
+      int first[4], last[4], v_top = kNoScale;
+      bool inside = true;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const Group q = group[g];
+        first[g] = max(0, from - q.base);
+        last[g] = min(to - q.base, q.valid - 1);
+        inside = inside && first[g] == 0 && last[g] == 15;
+        if (first[g] <= last[g]) v_top = max(v_top, q.v_exp);
+      }
+      const bool masks = !__all_sync(0xffffffffu, inside);
+      const int v_unit = v_top == kNoScale ? 0 : min(v_top + 1, 126);   // r = 2^v_unit
+      // the largest score of the tile
+      float most = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint32_t raw[16];
+        t_ld16(s_col + g * 16, raw);
+        t_wait_ld();
+        float top2[2] = {-INFINITY, -INFINITY};
+        if (masks) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i >= first[g] && i <= last[g]) top2[i & 1] = fmaxf(top2[i & 1], __uint_as_float(raw[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top2[i & 1] = fmaxf(top2[i & 1], __uint_as_float(raw[i]));
+        }
+        const float t = fmaxf(top2[0], top2[1]);
+        if (t > -INFINITY) most = fmaxf(most, t * (factor * group[g].k_scale));
+      }
+      float keep = 1.f;
+      if (most > top + kLag) {
+        keep = top == -INFINITY ? 1.f : exp2_fast(top - most);
+        top = most;
+      }
+      sum *= keep;
+      const float base = (top == -INFINITY ? 0.f : top) - kTopWeight;
+      // the tile before is multiplied out by now: fold it in, which frees its output and the columns of P
+      if (j > 0 && !fold(j - 1)) {
+        alive = false;
+        break;
+      }
+      fold_keep = keep;
+      fold_unit = exp2_fast((float)v_unit);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const Group q = group[g];
+        const float f = factor * q.k_scale;
+        // weights times V scale / r; a zero scale's codes are zero, so that any factor does
+        float shift = q.v_exp == kNoScale ? 0.f : (float)(q.v_exp - v_unit) + q.v_log;
+        if (shift < -100.f) shift = -100.f;   // 2^-100 of what the row sees beside it; not a number stays that
+        const float less = shift - base;
+        uint32_t raw[16], hi[8], lo[8];
+        t_ld16(s_col + g * 16, raw);
+        t_wait_ld();
+        float w[16], part[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = exp2_fast(fmaf(__uint_as_float(raw[i]), f, less));
+        if (masks) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = i >= first[g] && i <= last[g] ? w[i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[i & 1] += w[i];
+        if (!masks || first[g] <= last[g]) sum = fmaf(part[0] + part[1], exp2_fast(-shift), sum);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hi[i] = pack_f16(w[2 * i], w[2 * i + 1]);
+          if constexpr (PLANES == 2) lo[i] = pack_rest(w[2 * i], w[2 * i + 1], hi[i]);
+        }
+        __syncwarp();
+        t_st8(lane_addr + L::col_p + g * 8, hi);
+        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + 32 + g * 8, lo);
+      }
+      t_wait_st();
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(p_full);
+    }
+    if (alive && ntiles > 0) fold(ntiles - 1);
+    if (splits == 1) {
+      if (live) {
+#pragma unroll
+        for (int d = 0; d < HD; d += 4) store(local, head, d, make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]), sum);
+      }
+    } else {   // where the rings were: the last product has read them
+#pragma unroll
+      for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(s_out + m * L::line + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+      s_stat[m] = make_float2(top, sum);
+    }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    // ---- converters -----------------------------------------------------------------------------------------------------------
+    const int ct = (tid - 128) & 127, cw = (warp - 4) & 3, odd = (warp - 4) >> 2;
+    // K: half of a token's channels (HD bytes / 2); V: HD / 16 channels of eight tokens, a warp 32 neighbouring bytes at most of all 64
+    constexpr int KW = HD / 8, VW = HD / 64;   // words of K, words per token of V
+    const int k_token = ct >> 1, k_half = ct & 1, v_eight = lane & 7, v_part = (lane >> 3) + 4 * cw;
+    struct Place {   // 16 tokens: physical block (-1: none), place in it, first position
+      int id, sub, base;
+    };
+    auto locate = [&](int j, int group) -> Place {
+      const int q = (j * (int)splits + (int)split) * 4 + group, b = p.by_tiles(q);
+      Place at = {-1, (q - b * per_block) * 16, 0};
+      at.base = (first_block + b) * bs + at.sub;
+      if (j < ntiles && q < groups) at.id = __ldg(table + first_block + b);
+      return at;
+    };
+    struct Raw {
+      uint32_t k[KW], v[8][VW];
+      float2 k_scales;   // both scales of the group that this thread's token of K lies in
+      float v_scale;
+    };
+    auto fetch = [&](const Place& k_at, const Place& v_at, Raw& r) {
+#pragma unroll
+      for (int i = 0; i < KW; ++i) r.k[i] = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) r.v[t][w] = 0;
+      r.k_scales = make_float2(0.f, 0.f);
+      r.v_scale = 0.f;
+      if ((uint32_t)k_at.id < (uint32_t)p.num_blocks) {
+        const unsigned long long id = (uint32_t)k_at.id;
+        const uint8_t* k = p.codes + id * p.block_bytes + (size_t)kvh * 2 * p.side_bytes + (size_t)min(k_at.sub + (k_token & 15), bs - 1) * HD + k_half * (HD / 2);
+#pragma unroll
+        for (int i = 0; i < KW / 4; ++i) {
+          const uint4 v = __ldcs(reinterpret_cast<const uint4*>(k) + i);
+          r.k[4 * i] = v.x, r.k[4 * i + 1] = v.y, r.k[4 * i + 2] = v.z, r.k[4 * i + 3] = v.w;
+        }
+        r.k_scales = __ldg(reinterpret_cast<const float2*>(p.scales + (id * p.kv_heads + kvh) * 2));
+      }
+      if ((uint32_t)v_at.id < (uint32_t)p.num_blocks) {
+        const unsigned long long id = (uint32_t)v_at.id;
+        const uint8_t* v = p.codes + id * p.block_bytes + ((size_t)kvh * 2 + 1) * p.side_bytes + v_part * (HD / 16);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          // tokens that no row sees stay zero: their bytes may be anything, also what e4m3 calls NaN
+          const int off = (v_eight & 1) * 8 + t;
+          if (v_at.sub + off < bs && v_at.base + off >= lo_all && v_at.base + off <= hi_all) {
+            const uint8_t* at = v + (size_t)(v_at.sub + off) * HD;
+            if constexpr (VW == 2) {
+              const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
+              r.v[t][0] = x.x, r.v[t][1] = x.y;
+            } else {
+              r.v[t][0] = __ldcs(reinterpret_cast<const uint32_t*>(at));
+            }
+          }
+        }
+        r.v_scale = __ldg(p.scales + (id * p.kv_heads + kvh) * 2 + 1);
+      }
+    };
+    // a tile of this group's: what is in `cur`; the next one's codes are on their way, the one's behind it are being looked up
+    Raw cur, nxt;
+    Place k_here = locate(odd, k_token >> 4), v_next = locate(odd, v_eight >> 1), k_next = k_here;
+    fetch(k_here, v_next, cur);
+    k_next = locate(odd + 2, k_token >> 4);
+    v_next = locate(odd + 2, v_eight >> 1);
+    for (int j = odd; j < ntiles; j += 2) {
+      const int stg = j % kStagesP;
+      fetch(k_next, v_next, nxt);
+      const Place k_after = locate(j + 4, k_token >> 4);
+      v_next = locate(j + 4, v_eight >> 1);
+      if (!warp_wait(kv_free0 + 8 * stg, ((j / kStagesP) & 1) ^ 1, &s_abort, lane)) {
+        if (lane == 0) fail(23);
+        break;
+      }
+      unsigned char* kdst = smem + (size_t)stg * L::stage;
+      unsigned char* vdst = kdst + L::side;
+      if (lane == 0) {   // token 16 cw: this thread's token of K
+        Group q;
+        q.base = k_here.base;
+        q.valid = (uint32_t)k_here.id < (uint32_t)p.num_blocks ? min(16, bs - k_here.sub) : 0;
+        q.k_scale = cur.k_scales.x;
+        const float sv = cur.k_scales.y;
+        int e = 0;
+        const float mant = frexpf(sv, &e);   // [0.5, 1)
+        q.v_exp = sv == 0.f ? kNoScale : e - 1;
+        q.v_log = sv == 0.f ? 0.f : (sv < INFINITY ? log2f(2.f * mant) : NAN);
+        s_group[stg][cw] = q;
+      }
+      {   // K: two codes a word of f16, 16 bytes a store, [half of 64 channels][token][128 bytes] swizzled
+        constexpr int CHUNKS = KW / 2;   // of 8 channels
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          const uint32_t a = unsign<KIND>(cur.k[2 * c]), b = unsign<KIND>(cur.k[2 * c + 1]);
+          const uint4 x = make_uint4(widen<KIND, false>(a, false), widen<KIND, false>(a, true), widen<KIND, false>(b, false), widen<KIND, false>(b, true));
+          const int chunk = HD == 128 ? c : k_half * CHUNKS + c, sub = HD == 128 ? k_half : 0;
+          *reinterpret_cast<uint4*>(kdst + sub * 8192 + k_token * 128 + ((chunk ^ (k_token & 7)) << 4)) = x;
+        }
+      }
+      {   // V: eight tokens of a channel are 16 bytes, [channel][128 bytes] swizzled
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t u[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) u[t] = unsign<KIND>(cur.v_scale == 0.f ? 0 : cur.v[t][w]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t x[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[t] = __byte_perm(u[2 * t], u[2 * t + 1], half ? 0x7362 : 0x5140);
+#pragma unroll
+            for (int one = 0; one < 2; ++one) {
+              const int d = v_part * (HD / 16) + w * 4 + half * 2 + one;
+              const uint4 y = make_uint4(widen<KIND, false>(x[0], one), widen<KIND, false>(x[1], one), widen<KIND, false>(x[2], one), widen<KIND, false>(x[3], one));
+              *reinterpret_cast<uint4*>(vdst + d * 128 + ((v_eight ^ (d & 7)) << 4)) = y;
+            }
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic-proxy stores -> visible to the MMA's reads
+      __syncwarp();
+      if (lane == 0) bar_arrive(kv_full0 + 8 * stg);
+      cur = nxt;
+      k_here = k_next;
+      k_next = k_after;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 12 && pi_elect()) {
+    // ---- products ---------------------------------------------------------------------------------------------------------------
+    auto idesc = [](uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((uint32_t)(kRowsP >> 4) << 24); };   // f16 x f16 -> f32
+    auto scores = [&](int j) -> bool {
+      const int stg = j % kStagesP, buf = j & 1;
+      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / kStagesP) & 1)) {
+        fail(24);
+        return false;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t bd = desc_sw128(smem_base + stg * L::stage);
+#pragma unroll
+      for (int pl = PLANES - 1; pl >= 0; --pl)   // the smaller terms first
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+          mma_ts(tmem + L::col_s + buf * 64, tmem + L::col_q + pl * (HD / 2) + ks * 8, bd + (uint64_t)(((ks >> 2) * 8192 + (ks & 3) * 32) >> 4), idesc(kTileP),
+                 pl == PLANES - 1 && ks == 0 ? 0u : 1u);
+      mma_commit(s_full0 + 8 * buf);
+      return true;
+    };
+    bool ok = ntiles > 0 && scores(0);
+    for (int j = 0; j < ntiles && ok; ++j) {
+      const int stg = j % kStagesP;
+      // the next tile's scores run while the row threads work on this tile's
+      if (j + 1 < ntiles && !scores(j + 1)) break;
+      if (s_abort || !bar_wait(p_full, j & 1) || (j > 0 && !bar_wait(o_free, (j - 1) & 1))) {
+        fail(25);
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t bd = desc_sw128(smem_base + stg * L::stage + L::side);
+#pragma unroll
+      for (int pl = PLANES - 1; pl >= 0; --pl)
+#pragma unroll
+        for (int ks = 0; ks < kTileP / 16; ++ks)
+          mma_ts(tmem + L::col_o, tmem + L::col_p + pl * 32 + ks * 8, bd + (uint64_t)((ks * 32) >> 4), idesc(HD), pl == PLANES - 1 && ks == 0 ? 0u : 1u);
+      mma_commit(o_full);
+      mma_commit(kv_free0 + 8 * stg);
+    }
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 12) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+  if (splits == 1) return;
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int share = kRowsP / (int)splits, rows_here = min(pp.rows_per_tile, row_end - s_first);
+  for (int i = tid; i < share * (HD / 4); i += kThreadsP) {
+    const int mm = (int)split * share + i / (HD / 4), d = i % (HD / 4) * 4, row_local = p.by_group(mm);
+    if (row_local >= rows_here || d >= p.head_dim) continue;
+    float all = -INFINITY, l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t r = 0; r < splits; ++r) all = fmaxf(all, peer2(s_stat + mm, r).x);
+    for (uint32_t r = 0; r < splits; ++r) {
+      const float2 st = peer2(s_stat + mm, r);
+      const float4 x = peer4(s_out + mm * L::line + d, r);
+      const float f = join_factor(st.x, st.y, all);
+      v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+      l = fmaf(f, st.y, l);
+    }
+    store(row_local, mm - row_local * G, d, v, l);
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int KIND, int HD, int PLANES>
+pi_status launch_prefill(pi_ctx* ctx, const PrefillParams& p, dim3 grid, int splits) {
+  constexpr int bytes = Prefill<HD, PLANES>::smem;
+  auto kernel = kv8_prefill_kernel<KIND, HD, PLANES>;
+  static pi_smem_grant grant;
+  if (grant.of(ctx) == 0) {
+    PI_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    grant.of(ctx) = bytes;
+  }
+  PI_CUDA(ctx, pi_launch_chained(ctx, kernel, grid, dim3(kThreadsP), bytes, splits, p));
+  PI_CHECK_LAUNCH(ctx);
+  return PI_OK;
+}
+
+}  // namespace
+
+bool pi_kv8_prefill_takes(const pi_kv8_pool* pool, int group) { return (pool->pitch == 64 || pool->pitch == 128) && group <= kRowsP; }
+
+pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_kv8_attn_params& a, int min_cols, int max_context) {
+  PrefillParams p = {};
+  p.a = a;
+  p.rows_per_tile = kRowsP / a.group;
+  p.min_cols = min_cols;
+  p.err_flag = ctx->dev_err;
+  // tiles of rows: each sequence ends with one that may not be full
+  const long long full = (a.n_rows + p.rows_per_tile - 1) / p.rows_per_tile, most = full + std::min(a.n_seqs - 1, a.n_rows - 1);
+  PI_REQUIRE(ctx, most <= 65535, "%lld tiles of rows: at most 65535", most);
+  // few tiles share their positions out among clusters, four tiles of them or more to a CTA
+  const long long seen = a.window > 0 ? std::min<long long>(max_context, (long long)a.window + a.n_rows) : max_context;
+  int splits = 1;
+  while (splits < 8 && full * a.kv_heads * splits * 2 <= ctx->sm_count && seen / kTileP >= 4 * splits * 2) splits *= 2;
+  const dim3 grid((unsigned)(a.kv_heads * splits), (unsigned)most);
+  const bool two = a.dtype == PI_F32;
+  if (pool->kind == PI_INT8) {
+    if (pool->pitch == 64) return two ? launch_prefill<PI_INT8, 64, 2>(ctx, p, grid, splits) : launch_prefill<PI_INT8, 64, 1>(ctx, p, grid, splits);
+    return two ? launch_prefill<PI_INT8, 128, 2>(ctx, p, grid, splits) : launch_prefill<PI_INT8, 128, 1>(ctx, p, grid, splits);
+  }
+  if (pool->pitch == 64) return two ? launch_prefill<PI_E4M3, 64, 2>(ctx, p, grid, splits) : launch_prefill<PI_E4M3, 64, 1>(ctx, p, grid, splits);
+  return two ? launch_prefill<PI_E4M3, 128, 2>(ctx, p, grid, splits) : launch_prefill<PI_E4M3, 128, 1>(ctx, p, grid, splits);
+}
