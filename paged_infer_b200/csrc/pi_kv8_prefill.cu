@@ -315,22 +315,29 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       }
       const bool masks = !__all_sync(0xffffffffu, inside);
       const int v_unit = v_top == kNoScale ? 0 : min(v_top + 1, 126);   // r = 2^v_unit
+      float w[kTileP];
+      {
+        uint32_t raw[kTileP];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) t_ld16(s_col + g * 16, raw + g * 16);
+        t_wait_ld();
+#pragma unroll
+        for (int i = 0; i < kTileP; ++i) w[i] = __uint_as_float(raw[i]);
+      }
       // the largest score of the tile
       float most = -INFINITY;
+      if (masks) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t raw[16];
-        t_ld16(s_col + g * 16, raw);
-        t_wait_ld();
-        float top2[2] = {-INFINITY, -INFINITY};
-        if (masks) {
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (i >= first[g] && i <= last[g]) top2[i & 1] = fmaxf(top2[i & 1], __uint_as_float(raw[i]));
-        } else {
+            if (i < first[g] || i > last[g]) w[g * 16 + i] = -INFINITY;   // times the scale of K: still so, or not a number where that is none
+      }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top2[i & 1] = fmaxf(top2[i & 1], __uint_as_float(raw[i]));
-        }
+      for (int g = 0; g < 4; ++g) {
+        float top2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top2[i & 1] = fmaxf(top2[i & 1], w[g * 16 + i]);
         const float t = fmaxf(top2[0], top2[1]);
         if (t > -INFINITY) most = fmaxf(most, t * (factor * group[g].k_scale));
       }
@@ -341,6 +348,31 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       }
       sum *= keep;
       const float base = (top == -INFINITY ? 0.f : top) - kTopWeight;
+      uint32_t hi[kTileP / 2], lo[PLANES == 2 ? kTileP / 2 : 1];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const Group q = group[g];
+        const float f = factor * q.k_scale;
+        // weights times V scale / r; a zero scale's codes are zero, so that any factor does
+        float shift = q.v_exp == kNoScale ? 0.f : (float)(q.v_exp - v_unit) + q.v_log;
+        if (shift < -100.f) shift = -100.f;   // 2^-100 of what the row sees beside it; not a number stays that
+        const float less = shift - base;
+        float part[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[g * 16 + i] = exp2_fast(fmaf(w[g * 16 + i], f, less));
+        if (masks) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[g * 16 + i] = i >= first[g] && i <= last[g] ? w[g * 16 + i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[i & 1] += w[g * 16 + i];
+        if (!masks || first[g] <= last[g]) sum = fmaf(part[0] + part[1], exp2_fast(-shift), sum);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hi[g * 8 + i] = pack_f16(w[g * 16 + 2 * i], w[g * 16 + 2 * i + 1]);
+          if constexpr (PLANES == 2) lo[g * 8 + i] = pack_rest(w[g * 16 + 2 * i], w[g * 16 + 2 * i + 1], hi[g * 8 + i]);
+        }
+      }
       // the tile before is multiplied out by now: fold it in, which frees its output and the columns of P
       if (j > 0 && !fold(j - 1)) {
         alive = false;
@@ -350,33 +382,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       fold_unit = exp2_fast((float)v_unit);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const Group q = group[g];
-        const float f = factor * q.k_scale;
-        // weights times V scale / r; a zero scale's codes are zero, so that any factor does
-        float shift = q.v_exp == kNoScale ? 0.f : (float)(q.v_exp - v_unit) + q.v_log;
-        if (shift < -100.f) shift = -100.f;   // 2^-100 of what the row sees beside it; not a number stays that
-        const float less = shift - base;
-        uint32_t raw[16], hi[8], lo[8];
-        t_ld16(s_col + g * 16, raw);
-        t_wait_ld();
-        float w[16], part[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = exp2_fast(fmaf(__uint_as_float(raw[i]), f, less));
-        if (masks) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = i >= first[g] && i <= last[g] ? w[i] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[i & 1] += w[i];
-        if (!masks || first[g] <= last[g]) sum = fmaf(part[0] + part[1], exp2_fast(-shift), sum);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          hi[i] = pack_f16(w[2 * i], w[2 * i + 1]);
-          if constexpr (PLANES == 2) lo[i] = pack_rest(w[2 * i], w[2 * i + 1], hi[i]);
-        }
-        __syncwarp();
-        t_st8(lane_addr + L::col_p + g * 8, hi);
-        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + 32 + g * 8, lo);
+        t_st8(lane_addr + L::col_p + g * 8, hi + g * 8);
+        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + 32 + g * 8, lo + g * 8);
       }
       t_wait_st();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
