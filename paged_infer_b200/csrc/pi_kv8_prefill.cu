@@ -11,10 +11,12 @@
 // back, multiplied by r and added to the row's f32 output in registers.  The running maximum may lag 2^8 behind, so that the output
 // is hardly ever rescaled.
 //
-// Warps 0-3: a thread per row, with registers that the others give up.  Warps 4-7 and 8-11: the even and the odd tiles' codes, one of
-// theirs ahead in registers, then widened into shared memory (V by byte permutes of eight tokens at a time).  Warp 12: issues the
-// products (13-15 are there because registers are dealt to four warps at a time); the scores of tile j + 1 run while the rows work
-// on tile j.
+// Warps 0-7: two threads per row, each with half of a tile's columns and half of the output's channels; they share the row's running
+// maximum through shared memory, once a tile.  (One thread per row left every scheduler one such warp, and nothing to do while that
+// waited for tensor memory, the exponential or its next instructions: 1.7 times the time.)  Warps 8-11 and 12-15: the even and the odd
+// tiles' codes, into registers ahead of their turn, then widened into shared memory (V by byte permutes of eight tokens at a time).
+// Warp 16: issues the products (17-19 are there because registers are dealt to four warps at a time); the scores of tile j + 1 run
+// while the rows work on tile j.
 // Hand-offs go through mbarriers; every wait is bounded and raises the context's error word instead of hanging.  Where there are few
 // tiles of rows, a cluster shares the positions of one and joins its CTAs' outputs through shared memory.
 //
@@ -31,8 +33,8 @@ namespace {
 
 using namespace pi_kv8;
 
-constexpr int kRowsP = 128, kTileP = 64, kThreadsP = 16 * 32, kStagesP = 4;
-constexpr uint32_t kSpinP = 1u << 20, kNap = 256;   // polls, and the nanoseconds that each may sleep
+constexpr int kRowsP = 128, kTileP = 64, kThreadsP = 20 * 32, kStagesP = 4;
+constexpr uint32_t kSpinP = 1u << 21;   // polls of a wait
 
 struct PrefillParams {
   pi_kv8_attn_params a;
@@ -52,17 +54,21 @@ constexpr int kNoScale = -100000;   // v_exp of a zero scale
 __device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Polls while others wait for this thread; converters, who are ahead, sleep between theirs.
+template <bool NAP = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t spin = 0; spin < kSpinP; ++spin) {
+  for (uint32_t spin = 0; spin < (NAP ? kSpinP >> 3 : kSpinP); ++spin) {
     uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity), "r"(kNap) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
+    if (NAP) __nanosleep(64);
   }
   return false;
 }
+template <bool NAP = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int lane) {
   int ok = 1;
-  if (lane == 0) ok = (!*abort_flag && bar_wait(bar, parity)) ? 1 : 0;
+  if (lane == 0) ok = (!*abort_flag && bar_wait<NAP>(bar, parity)) ? 1 : 0;
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 // K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
@@ -112,6 +118,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   __shared__ Group s_group[kStagesP][4];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
+  __shared__ float s_most[2][2][kRowsP];   // [tile parity][half][row]
   __shared__ int s_lo, s_hi, s_seq, s_first;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = p.block_size, G = p.group;
@@ -161,9 +168,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         bar_init(kv_free0 + 8 * i, 1);   // tcgen05.commit
       }
       for (int i = 0; i < 2; ++i) bar_init(s_full0 + 8 * i, 1);
-      bar_init(p_full, 4);               // one arrival per row warp
+      bar_init(p_full, 8);               // one arrival per row warp
       bar_init(o_full, 1);
-      bar_init(o_free, 4);
+      bar_init(o_free, 8);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -171,13 +178,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   __syncthreads();
   const int seq = s_seq;
   if (seq < 0) return;   // the whole cluster: fewer tiles than the grid allows for
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&s_tmem)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // this thread's row (warps 0-3)
-  const int row_end = min(p.cu_rows[seq + 1], p.n_rows), m = tid, local = p.by_group(m), head = m - local * G;
-  const bool live = warp < 4 && local < pp.rows_per_tile && s_first + local < row_end;
+  // this thread's row (warps 0-7), and its half of it
+  const int row_end = min(p.cu_rows[seq + 1], p.n_rows), m = tid & 127, half = tid >> 7, local = p.by_group(m), head = m - local * G;
+  const bool live = warp < 8 && local < pp.rows_per_tile && s_first + local < row_end;
   int pos = -1, from = 0;
   if (live) {
     pos = p.row_pos[s_first + local];
@@ -202,8 +209,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
 
   float factor = 0.f;
-  if (warp < 4) {
-    // the row's query: two readings, the largest channel first
+  if (warp < 8) {
+    // the row's query, half of its channels a thread: two readings, the largest channel first
     const size_t at = live ? (size_t)(s_first + local) * p.q_stride + (size_t)(kvh * G + head) * p.head_dim : 0;
     float most = 0.f;
 #pragma unroll 4
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     const float shrink = __uint_as_float((253u - e) << 23);
     factor = __uint_as_float((e + 1) << 23) * p.scale2;
 #pragma unroll 2
-    for (int d = 0; d < HD; d += 16) {
+    for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 16) {
       uint32_t hi[8], lo[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -255,14 +262,14 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     if (d < p.head_dim)
       pi_store4_f32_as(y, p.out, (size_t)(s_first + row_local) * p.out_stride + (size_t)(kvh * G + h) * p.head_dim + d, p.dtype, p.head_dim - d, p.out_wide);
   };
-  // of the 512 registers that four warps of a lane's number have at launch, one of each group: 240 for a row, 96 for each group of
-  // converters, 80 for the rest
-  if (warp < 4) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
-    float acc[HD], top = -INFINITY, sum = 0.f;
+  // of the 5 x 96 registers that the groups of four warps have at launch: 144 for each of rows, 72 for each of converters, 48 for the rest
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    constexpr int HALF = HD / 2;   // channels of this thread
+    float acc[HALF], top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD; ++i) acc[i] = 0.f;
-    // ---- a thread per row ---------------------------------------------------------------------------------------------------
+    for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+    // ---- rows -----------------------------------------------------------------------------------------------------------------
     float fold_keep = 1.f, fold_unit = 0.f;   // of the tile before: what became of the output so far, and its r
     bool alive = true;
     const int to = min(pos, hi_all);
@@ -274,10 +281,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool shrunk = __any_sync(0xffffffffu, fold_keep != 1.f);
 #pragma unroll
-      for (int c = 0; c < HD; c += 32) {
+      for (int c = 0; c < HALF; c += 32) {
         uint32_t o[32];
-        t_ld16(lane_addr + L::col_o + c, o);
-        t_ld16(lane_addr + L::col_o + c + 16, o + 16);
+        t_ld16(lane_addr + L::col_o + half * HALF + c, o);
+        t_ld16(lane_addr + L::col_o + half * HALF + c + 16, o + 16);
         t_wait_ld();
         if (shrunk) {
 #pragma unroll
@@ -291,56 +298,69 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       if (lane == 0) bar_arrive(o_free);
       return true;
     };
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };   // the two halves' warps: once a tile, come what may
     for (int j = 0; j < ntiles; ++j) {
       const int buf = j & 1;
+      if (!alive) {
+        meet();
+        continue;
+      }
       // the scores, and for the groups' scales what the converters released with the codes (this phase cannot pass before P is handed over)
       if (!warp_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort, lane) || !warp_wait(kv_full0 + 8 * (j % kStagesP), (j / kStagesP) & 1, &s_abort, lane)) {
         if (lane == 0) fail(21);
         alive = false;
-        break;
+        meet();
+        continue;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const Group* group = s_group[j % kStagesP];
-      const uint32_t s_col = lane_addr + L::col_s + buf * 64;
-      // what the row sees of each group: its columns first .. last
-      int first[4], last[4], v_top = kNoScale;
+      const uint32_t s_col = lane_addr + L::col_s + buf * 64 + half * 32;
+      // what the row sees of this thread's groups: their columns first .. last; r goes by all four
+      int first[2], last[2], v_top = kNoScale;
       bool inside = true;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const Group q = group[g];
-        first[g] = max(0, from - q.base);
-        last[g] = min(to - q.base, q.valid - 1);
-        inside = inside && first[g] == 0 && last[g] == 15;
-        if (first[g] <= last[g]) v_top = max(v_top, q.v_exp);
+        const int f = max(0, from - q.base), l = min(to - q.base, q.valid - 1);
+        if (f <= l) v_top = max(v_top, q.v_exp);
+        if (g >> 1 == half) {
+          first[g & 1] = f;
+          last[g & 1] = l;
+          inside = inside && f == 0 && l == 15;
+        }
       }
       const bool masks = !__all_sync(0xffffffffu, inside);
       const int v_unit = v_top == kNoScale ? 0 : min(v_top + 1, 126);   // r = 2^v_unit
-      float w[kTileP];
+      float w[kTileP / 2];
       {
-        uint32_t raw[kTileP];
+        uint32_t raw[kTileP / 2];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) t_ld16(s_col + g * 16, raw + g * 16);
+        for (int g = 0; g < 2; ++g) t_ld16(s_col + g * 16, raw + g * 16);
         t_wait_ld();
 #pragma unroll
-        for (int i = 0; i < kTileP; ++i) w[i] = __uint_as_float(raw[i]);
+        for (int i = 0; i < kTileP / 2; ++i) w[i] = __uint_as_float(raw[i]);
       }
       // the largest score of the tile
       float most = -INFINITY;
       if (masks) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (i < first[g] || i > last[g]) w[g * 16 + i] = -INFINITY;   // times the scale of K: still so, or not a number where that is none
       }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2; ++g) {
         float top2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 16; ++i) top2[i & 1] = fmaxf(top2[i & 1], w[g * 16 + i]);
         const float t = fmaxf(top2[0], top2[1]);
-        if (t > -INFINITY) most = fmaxf(most, t * (factor * group[g].k_scale));
+        if (t > -INFINITY) most = fmaxf(most, t * (factor * group[half * 2 + g].k_scale));
       }
+      // the other half's; both threads come to the same maximum
+      s_most[buf][half][m] = most;
+      meet();
+      most = fmaxf(most, s_most[buf][half ^ 1][m]);
       float keep = 1.f;
       if (most > top + kLag) {
         keep = top == -INFINITY ? 1.f : exp2_fast(top - most);
@@ -348,10 +368,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       }
       sum *= keep;
       const float base = (top == -INFINITY ? 0.f : top) - kTopWeight;
-      uint32_t hi[kTileP / 2], lo[PLANES == 2 ? kTileP / 2 : 1];
+      uint32_t hi[kTileP / 4], lo[PLANES == 2 ? kTileP / 4 : 1];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const Group q = group[g];
+      for (int g = 0; g < 2; ++g) {
+        const Group q = group[half * 2 + g];
         const float f = factor * q.k_scale;
         // weights times V scale / r; a zero scale's codes are zero, so that any factor does
         float shift = q.v_exp == kNoScale ? 0.f : (float)(q.v_exp - v_unit) + q.v_log;
@@ -376,14 +396,14 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       // the tile before is multiplied out by now: fold it in, which frees its output and the columns of P
       if (j > 0 && !fold(j - 1)) {
         alive = false;
-        break;
+        continue;
       }
       fold_keep = keep;
       fold_unit = exp2_fast((float)v_unit);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        t_st8(lane_addr + L::col_p + g * 8, hi + g * 8);
-        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + 32 + g * 8, lo + g * 8);
+      for (int g = 0; g < 2; ++g) {
+        t_st8(lane_addr + L::col_p + half * 16 + g * 8, hi + g * 8);
+        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + 32 + half * 16 + g * 8, lo + g * 8);
       }
       t_wait_st();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -391,20 +411,24 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       if (lane == 0) bar_arrive(p_full);
     }
     if (alive && ntiles > 0) fold(ntiles - 1);
+    // the halves' sums, in the buffer that the last tile did not use
+    s_most[ntiles & 1][half][m] = sum;
+    meet();
+    sum = s_most[ntiles & 1][0][m] + s_most[ntiles & 1][1][m];
     if (splits == 1) {
       if (live) {
 #pragma unroll
-        for (int d = 0; d < HD; d += 4) store(local, head, d, make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]), sum);
+        for (int d = 0; d < HALF; d += 4) store(local, head, half * HALF + d, make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]), sum);
       }
     } else {   // where the rings were: the last product has read them
 #pragma unroll
-      for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(s_out + m * L::line + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-      s_stat[m] = make_float2(top, sum);
+      for (int d = 0; d < HALF; d += 4) *reinterpret_cast<float4*>(s_out + m * L::line + half * HALF + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+      if (half == 0) s_stat[m] = make_float2(top, sum);
     }
-  } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ---- converters -----------------------------------------------------------------------------------------------------------
-    const int ct = (tid - 128) & 127, cw = (warp - 4) & 3, odd = (warp - 4) >> 2;
+    const int ct = tid & 127, cw = warp & 3, odd = (warp - 8) >> 2;
     // K: half of a token's channels (HD bytes / 2); V: HD / 16 channels of eight tokens, a warp 32 neighbouring bytes at most of all 64
     constexpr int KW = HD / 8, VW = HD / 64;   // words of K, words per token of V
     const int k_token = ct >> 1, k_half = ct & 1, v_eight = lane & 7, v_part = (lane >> 3) + 4 * cw;
@@ -462,18 +486,15 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         r.v_scale = __ldg(p.scales + (id * p.kv_heads + kvh) * 2 + 1);
       }
     };
-    // a tile of this group's: what is in `cur`; the next one's codes are on their way, the one's behind it are being looked up
-    Raw cur, nxt;
-    Place k_here = locate(odd, k_token >> 4), v_next = locate(odd, v_eight >> 1), k_next = k_here;
-    fetch(k_here, v_next, cur);
-    k_next = locate(odd + 2, k_token >> 4);
-    v_next = locate(odd + 2, v_eight >> 1);
+    // the codes of a tile are requested as soon as this group's one before is stored, its table entries one tile earlier
+    Raw cur;
+    Place k_here = locate(odd, k_token >> 4), v_here = locate(odd, v_eight >> 1);
+    fetch(k_here, v_here, cur);
     for (int j = odd; j < ntiles; j += 2) {
       const int stg = j % kStagesP;
-      fetch(k_next, v_next, nxt);
-      const Place k_after = locate(j + 4, k_token >> 4);
-      v_next = locate(j + 4, v_eight >> 1);
-      if (!warp_wait(kv_free0 + 8 * stg, ((j / kStagesP) & 1) ^ 1, &s_abort, lane)) {
+      const Place k_next = locate(j + 2, k_token >> 4);
+      v_here = locate(j + 2, v_eight >> 1);
+      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / kStagesP) & 1) ^ 1, &s_abort, lane)) {
         if (lane == 0) fail(23);
         break;
       }
@@ -524,13 +545,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // generic-proxy stores -> visible to the MMA's reads
       __syncwarp();
       if (lane == 0) bar_arrive(kv_full0 + 8 * stg);
-      cur = nxt;
       k_here = k_next;
-      k_next = k_after;
+      if (j + 2 < ntiles) fetch(k_here, v_here, cur);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 12 && pi_elect()) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 16)
+      if (pi_elect()) {   // a test of its own: behind a compound one the descriptors do not stay in uniform registers
     // ---- products ---------------------------------------------------------------------------------------------------------------
     auto idesc = [](uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((uint32_t)(kRowsP >> 4) << 24); };   // f16 x f16 -> f32
     auto scores = [&](int j) -> bool {
@@ -574,7 +595,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
