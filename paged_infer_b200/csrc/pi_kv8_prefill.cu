@@ -2,7 +2,7 @@
 // operands in tensor memory, B operands in shared memory.  Head sizes that are stored in 64 or 128 bytes.
 //
 // A CTA owns 128 (row, query head) pairs of one sequence and KV head, one per TMEM lane, and walks the positions that they see in tiles
-// of 64 columns: four times 16 tokens, each of one block and with one pair of scales.  Codes are widened to f16, which holds them
+// of 128 columns (64 for heads of 128 with two planes): eight times 16 tokens, each of one block and with one pair of scales.  Codes are widened to f16, which holds them
 // exactly; queries (brought to [-1, 1] by a power of two per row) and weights are f16 too, in two planes (22 bits) for f32 tensors:
 //     scores  S = Q K^T        A = Q (written once),  B = codes of K, [token][channel]
 //     output  O = P V          A = P,                 B = codes of V transposed, [channel][token]
@@ -33,7 +33,7 @@ namespace {
 
 using namespace pi_kv8;
 
-constexpr int kRowsP = 128, kTileP = 64, kThreadsP = 20 * 32, kStagesP = 4;
+constexpr int kRowsP = 128, kPartP = 64, kThreadsP = 20 * 32, kMostStages = 4;   // a part: the tokens of a tile that four warps widen
 constexpr uint32_t kSpinP = 1u << 21;   // polls of a wait
 
 struct PrefillParams {
@@ -54,21 +54,21 @@ constexpr int kNoScale = -100000;   // v_exp of a zero scale
 __device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// Polls while others wait for this thread; converters, who are ahead, sleep between theirs.
-template <bool NAP = false>
+// A try may suspend the thread for a while that the hardware limits; tries end after kSpinP of them or about a second.  (Polling with
+// test_wait, 700 times a tile and SM, cost a third of the issue slots and made every wait on a barrier 400 clocks long.)
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t spin = 0; spin < (NAP ? kSpinP >> 3 : kSpinP); ++spin) {
+  const long long until = clock64() + (1ll << 31);
+  for (uint32_t spin = 0; spin < kSpinP; ++spin) {
     uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
-    if (NAP) __nanosleep(64);
+    if (clock64() > until) return false;
   }
   return false;
 }
-template <bool NAP = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int lane) {
   int ok = 1;
-  if (lane == 0) ok = (!*abort_flag && bar_wait<NAP>(bar, parity)) ? 1 : 0;
+  if (lane == 0) ok = (!*abort_flag && bar_wait(bar, parity)) ? 1 : 0;
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 // K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
@@ -98,24 +98,29 @@ __device__ __forceinline__ void t_wait_st() { asm volatile("tcgen05.wait::st.syn
 
 template <int HD, int PLANES>
 struct Prefill {
-  static constexpr int side = kTileP * HD * 2, stage = 2 * side;   // bytes of a tile's K, and as many of V
+  // columns of a tile: two buffers of scores, P, the output and Q have to fit the 512 columns of tensor memory
+  static constexpr int tile = HD == 128 && PLANES == 2 ? 64 : 128, parts = tile / kPartP, groups = tile / 16;
+  static constexpr int side = tile * HD * 2, stage = 2 * side;     // bytes of a tile's K, and as many of V
+  static constexpr int stages = stage > 32768 ? 3 : 4;
   static constexpr int line = HD + 4;                              // floats of a row where the CTAs of a cluster meet
-  static constexpr int rings = kStagesP * stage, meet = kRowsP * line * 4 + kRowsP * 8;
+  static constexpr int rings = stages * stage, meet = kRowsP * line * 4 + kRowsP * 8;
   static constexpr int body = rings > meet ? rings : meet;
   // at least 120 KB: two of these CTAs, each of which takes all of tensor memory, never share an SM
   static constexpr int smem = (body > 119 * 1024 ? body : 119 * 1024) + 1024;
   // tensor memory: two buffers of scores, the planes of P, the tile's output, the planes of Q
-  static constexpr uint32_t col_s = 0, col_p = 128, col_o = 192, col_q = 320;
+  static constexpr uint32_t col_s = 0, col_p = 2 * tile, col_o = col_p + PLANES * tile / 2, col_q = col_o + HD;
+  static_assert(col_q + PLANES * HD / 2 <= 512, "tensor memory");
 };
 
 template <int KIND, int HD, int PLANES>
 __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const PrefillParams pp) {
   using L = Prefill<HD, PLANES>;
+  constexpr int TILE = L::tile, STAGES = L::stages, PARTS = L::parts;
   const pi_kv8_attn_params& p = pp.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) unsigned long long bars[2 * kStagesP + 5];
-  __shared__ Group s_group[kStagesP][4];
+  __shared__ __align__(8) unsigned long long bars[2 * kMostStages + 5];
+  __shared__ Group s_group[kMostStages][8];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ float s_most[2][2][kRowsP];   // [tile parity][half][row]
@@ -126,8 +131,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const int kvh = blockIdx.x / splits;
-  const uint32_t kv_full0 = s_u32(&bars[0]), kv_free0 = s_u32(&bars[kStagesP]), s_full0 = s_u32(&bars[2 * kStagesP]), p_full = s_u32(&bars[2 * kStagesP + 2]),
-                 o_full = s_u32(&bars[2 * kStagesP + 3]), o_free = s_u32(&bars[2 * kStagesP + 4]);
+  const uint32_t kv_full0 = s_u32(&bars[0]), kv_free0 = s_u32(&bars[kMostStages]), s_full0 = s_u32(&bars[2 * kMostStages]), p_full = s_u32(&bars[2 * kMostStages + 2]),
+                 o_full = s_u32(&bars[2 * kMostStages + 3]), o_free = s_u32(&bars[2 * kMostStages + 4]);
   pi_grid_dependency_wait_only();
 
   // the tile of rows: sequences' tiles are numbered through
@@ -163,8 +168,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       s_lo = 0x7fffffff;
       s_hi = -1;
       s_abort = 0;
-      for (int i = 0; i < kStagesP; ++i) {
-        bar_init(kv_full0 + 8 * i, 4);   // one arrival per converter warp
+      for (int i = 0; i < L::stages; ++i) {
+        bar_init(kv_full0 + 8 * i, 4 * L::parts);   // one arrival per converter warp
         bar_init(kv_free0 + 8 * i, 1);   // tcgen05.commit
       }
       for (int i = 0; i < 2; ++i) bar_init(s_full0 + 8 * i, 1);
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   const uint32_t tmem = s_tmem, smem_base = s_u32(smem), lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   const int lo_all = s_lo, hi_all = min(s_hi, (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1);
   const int per_block = (bs + 15) >> 4, first_block = hi_all < lo_all ? 0 : p.by_block(lo_all);
-  const int groups = hi_all < lo_all ? 0 : (p.by_block(hi_all) - first_block + 1) * per_block, tiles_all = (groups + 3) >> 2;
+  const int groups = hi_all < lo_all ? 0 : (p.by_block(hi_all) - first_block + 1) * per_block, tiles_all = (groups + L::groups - 1) / L::groups;
   // this CTA's share of the positions: every splits-th tile
   const int ntiles = tiles_all > (int)split ? (tiles_all - (int)split + (int)splits - 1) / (int)splits : 0;
   const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
@@ -262,9 +267,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     if (d < p.head_dim)
       pi_store4_f32_as(y, p.out, (size_t)(s_first + row_local) * p.out_stride + (size_t)(kvh * G + h) * p.head_dim + d, p.dtype, p.head_dim - d, p.out_wide);
   };
-  // of the 5 x 96 registers that the groups of four warps have at launch: 144 for each of rows, 72 for each of converters, 48 for the rest
+  // of the 5 x 96 registers that the groups of four warps have at launch: 152 for each of rows, 64 for each of converters, 48 for the rest
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     constexpr int HALF = HD / 2;   // channels of this thread
     float acc[HALF], top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -305,57 +310,58 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         meet();
         continue;
       }
-      // the scores, and for the groups' scales what the converters released with the codes (this phase cannot pass before P is handed over)
-      if (!warp_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort, lane) || !warp_wait(kv_full0 + 8 * (j % kStagesP), (j / kStagesP) & 1, &s_abort, lane)) {
+      // the scores; what the converters wrote of the groups was released to the thread that issued them
+      if (!warp_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort, lane)) {
         if (lane == 0) fail(21);
         alive = false;
         meet();
         continue;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const Group* group = s_group[j % kStagesP];
-      const uint32_t s_col = lane_addr + L::col_s + buf * 64 + half * 32;
-      // what the row sees of this thread's groups: their columns first .. last; r goes by all four
-      int first[2], last[2], v_top = kNoScale;
+      const Group* group = s_group[j % STAGES];
+      constexpr int COLS = TILE / 2, GROUPS = COLS / 16;   // of this thread
+      const uint32_t s_col = lane_addr + L::col_s + buf * TILE + half * COLS;
+      // what the row sees of this thread's groups: their columns first .. last; r goes by all
+      int first[GROUPS], last[GROUPS], v_top = kNoScale;
       bool inside = true;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2 * GROUPS; ++g) {
         const Group q = group[g];
         const int f = max(0, from - q.base), l = min(to - q.base, q.valid - 1);
         if (f <= l) v_top = max(v_top, q.v_exp);
-        if (g >> 1 == half) {
-          first[g & 1] = f;
-          last[g & 1] = l;
+        if (g / GROUPS == half) {
+          first[g % GROUPS] = f;
+          last[g % GROUPS] = l;
           inside = inside && f == 0 && l == 15;
         }
       }
       const bool masks = !__all_sync(0xffffffffu, inside);
       const int v_unit = v_top == kNoScale ? 0 : min(v_top + 1, 126);   // r = 2^v_unit
-      float w[kTileP / 2];
+      float w[COLS];
       {
-        uint32_t raw[kTileP / 2];
+        uint32_t raw[COLS];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) t_ld16(s_col + g * 16, raw + g * 16);
+        for (int g = 0; g < GROUPS; ++g) t_ld16(s_col + g * 16, raw + g * 16);
         t_wait_ld();
 #pragma unroll
-        for (int i = 0; i < kTileP / 2; ++i) w[i] = __uint_as_float(raw[i]);
+        for (int i = 0; i < COLS; ++i) w[i] = __uint_as_float(raw[i]);
       }
       // the largest score of the tile
       float most = -INFINITY;
       if (masks) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (i < first[g] || i > last[g]) w[g * 16 + i] = -INFINITY;   // times the scale of K: still so, or not a number where that is none
       }
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int g = 0; g < GROUPS; ++g) {
         float top2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 16; ++i) top2[i & 1] = fmaxf(top2[i & 1], w[g * 16 + i]);
         const float t = fmaxf(top2[0], top2[1]);
-        if (t > -INFINITY) most = fmaxf(most, t * (factor * group[half * 2 + g].k_scale));
+        if (t > -INFINITY) most = fmaxf(most, t * (factor * group[half * GROUPS + g].k_scale));
       }
       // the other half's; both threads come to the same maximum
       s_most[buf][half][m] = most;
@@ -368,10 +374,10 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       }
       sum *= keep;
       const float base = (top == -INFINITY ? 0.f : top) - kTopWeight;
-      uint32_t hi[kTileP / 4], lo[PLANES == 2 ? kTileP / 4 : 1];
+      uint32_t hi[COLS / 2], lo[PLANES == 2 ? COLS / 2 : 1];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const Group q = group[half * 2 + g];
+      for (int g = 0; g < GROUPS; ++g) {
+        const Group q = group[half * GROUPS + g];
         const float f = factor * q.k_scale;
         // weights times V scale / r; a zero scale's codes are zero, so that any factor does
         float shift = q.v_exp == kNoScale ? 0.f : (float)(q.v_exp - v_unit) + q.v_log;
@@ -401,9 +407,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       fold_keep = keep;
       fold_unit = exp2_fast((float)v_unit);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        t_st8(lane_addr + L::col_p + half * 16 + g * 8, hi + g * 8);
-        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + 32 + half * 16 + g * 8, lo + g * 8);
+      for (int g = 0; g < GROUPS; ++g) {
+        t_st8(lane_addr + L::col_p + half * (COLS / 2) + g * 8, hi + g * 8);
+        if constexpr (PLANES == 2) t_st8(lane_addr + L::col_p + TILE / 2 + half * (COLS / 2) + g * 8, lo + g * 8);
       }
       t_wait_st();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -426,9 +432,11 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       if (half == 0) s_stat[m] = make_float2(top, sum);
     }
   } else if (warp < 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ---- converters -----------------------------------------------------------------------------------------------------------
-    const int ct = tid & 127, cw = warp & 3, odd = (warp - 8) >> 2;
+    const int ct = tid & 127, cw = warp & 3, which = (warp - 8) >> 2;   // of two: a part of every tile, or every other tile of one part
+    constexpr int EVERY = PARTS == 2 ? 1 : 2;
+    const int part = PARTS == 2 ? which : 0, j0 = PARTS == 2 ? 0 : which;
     // K: half of a token's channels (HD bytes / 2); V: HD / 16 channels of eight tokens, a warp 32 neighbouring bytes at most of all 64
     constexpr int KW = HD / 8, VW = HD / 64;   // words of K, words per token of V
     const int k_token = ct >> 1, k_half = ct & 1, v_eight = lane & 7, v_part = (lane >> 3) + 4 * cw;
@@ -436,7 +444,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       int id, sub, base;
     };
     auto locate = [&](int j, int group) -> Place {
-      const int q = (j * (int)splits + (int)split) * 4 + group, b = p.by_tiles(q);
+      const int q = (j * (int)splits + (int)split) * L::groups + part * 4 + group, b = p.by_tiles(q);
       Place at = {-1, (q - b * per_block) * 16, 0};
       at.base = (first_block + b) * bs + at.sub;
       if (j < ntiles && q < groups) at.id = __ldg(table + first_block + b);
@@ -488,13 +496,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     };
     // the codes of a tile are requested as soon as this group's one before is stored, its table entries one tile earlier
     Raw cur;
-    Place k_here = locate(odd, k_token >> 4), v_here = locate(odd, v_eight >> 1);
+    Place k_here = locate(j0, k_token >> 4), v_here = locate(j0, v_eight >> 1);
     fetch(k_here, v_here, cur);
-    for (int j = odd; j < ntiles; j += 2) {
-      const int stg = j % kStagesP;
-      const Place k_next = locate(j + 2, k_token >> 4);
-      v_here = locate(j + 2, v_eight >> 1);
-      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / kStagesP) & 1) ^ 1, &s_abort, lane)) {
+    for (int j = j0; j < ntiles; j += EVERY) {
+      const int stg = j % STAGES;
+      const Place k_next = locate(j + EVERY, k_token >> 4);
+      v_here = locate(j + EVERY, v_eight >> 1);
+      if (!warp_wait(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort, lane)) {
         if (lane == 0) fail(23);
         break;
       }
@@ -510,19 +518,19 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         const float mant = frexpf(sv, &e);   // [0.5, 1)
         q.v_exp = sv == 0.f ? kNoScale : e - 1;
         q.v_log = sv == 0.f ? 0.f : (sv < INFINITY ? log2f(2.f * mant) : NAN);
-        s_group[stg][cw] = q;
+        s_group[stg][part * 4 + cw] = q;
       }
-      {   // K: two codes a word of f16, 16 bytes a store, [half of 64 channels][token][128 bytes] swizzled
+      {   // K: two codes a word of f16, 16 bytes a store, [64 channels][token][128 bytes] swizzled
         constexpr int CHUNKS = KW / 2;   // of 8 channels
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           const uint32_t a = unsign<KIND>(cur.k[2 * c]), b = unsign<KIND>(cur.k[2 * c + 1]);
           const uint4 x = make_uint4(widen<KIND, false>(a, false), widen<KIND, false>(a, true), widen<KIND, false>(b, false), widen<KIND, false>(b, true));
           const int chunk = HD == 128 ? c : k_half * CHUNKS + c, sub = HD == 128 ? k_half : 0;
-          *reinterpret_cast<uint4*>(kdst + sub * 8192 + k_token * 128 + ((chunk ^ (k_token & 7)) << 4)) = x;
+          *reinterpret_cast<uint4*>(kdst + sub * (TILE * 128) + (part * kPartP + k_token) * 128 + ((chunk ^ (k_token & 7)) << 4)) = x;
         }
       }
-      {   // V: eight tokens of a channel are 16 bytes, [channel][128 bytes] swizzled
+      {   // V: eight tokens of a channel are 16 bytes, [part][channel][128 bytes] swizzled
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t u[8];
@@ -537,7 +545,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
             for (int one = 0; one < 2; ++one) {
               const int d = v_part * (HD / 16) + w * 4 + half * 2 + one;
               const uint4 y = make_uint4(widen<KIND, false>(x[0], one), widen<KIND, false>(x[1], one), widen<KIND, false>(x[2], one), widen<KIND, false>(x[3], one));
-              *reinterpret_cast<uint4*>(vdst + d * 128 + ((v_eight ^ (d & 7)) << 4)) = y;
+              *reinterpret_cast<uint4*>(vdst + part * (HD * 128) + d * 128 + ((v_eight ^ (d & 7)) << 4)) = y;
             }
           }
         }
@@ -546,7 +554,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       __syncwarp();
       if (lane == 0) bar_arrive(kv_full0 + 8 * stg);
       k_here = k_next;
-      if (j + 2 < ntiles) fetch(k_here, v_here, cur);
+      if (j + EVERY < ntiles) fetch(k_here, v_here, cur);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
@@ -555,8 +563,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     // ---- products ---------------------------------------------------------------------------------------------------------------
     auto idesc = [](uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((uint32_t)(kRowsP >> 4) << 24); };   // f16 x f16 -> f32
     auto scores = [&](int j) -> bool {
-      const int stg = j % kStagesP, buf = j & 1;
-      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / kStagesP) & 1)) {
+      const int stg = j % STAGES, buf = j & 1;
+      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / STAGES) & 1)) {
         fail(24);
         return false;
       }
@@ -566,14 +574,14 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       for (int pl = PLANES - 1; pl >= 0; --pl)   // the smaller terms first
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks)
-          mma_ts(tmem + L::col_s + buf * 64, tmem + L::col_q + pl * (HD / 2) + ks * 8, bd + (uint64_t)(((ks >> 2) * 8192 + (ks & 3) * 32) >> 4), idesc(kTileP),
+          mma_ts(tmem + L::col_s + buf * TILE, tmem + L::col_q + pl * (HD / 2) + ks * 8, bd + (uint64_t)(((ks >> 2) * (TILE * 128) + (ks & 3) * 32) >> 4), idesc(TILE),
                  pl == PLANES - 1 && ks == 0 ? 0u : 1u);
       mma_commit(s_full0 + 8 * buf);
       return true;
     };
     bool ok = ntiles > 0 && scores(0);
     for (int j = 0; j < ntiles && ok; ++j) {
-      const int stg = j % kStagesP;
+      const int stg = j % STAGES;
       // the next tile's scores run while the row threads work on this tile's
       if (j + 1 < ntiles && !scores(j + 1)) break;
       if (s_abort || !bar_wait(p_full, j & 1) || (j > 0 && !bar_wait(o_free, (j - 1) & 1))) {
@@ -585,8 +593,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 #pragma unroll
       for (int pl = PLANES - 1; pl >= 0; --pl)
 #pragma unroll
-        for (int ks = 0; ks < kTileP / 16; ++ks)
-          mma_ts(tmem + L::col_o, tmem + L::col_p + pl * 32 + ks * 8, bd + (uint64_t)((ks * 32) >> 4), idesc(HD), pl == PLANES - 1 && ks == 0 ? 0u : 1u);
+        for (int ks = 0; ks < TILE / 16; ++ks)
+          mma_ts(tmem + L::col_o, tmem + L::col_p + pl * (TILE / 2) + ks * 8, bd + (uint64_t)(((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc(HD), pl == PLANES - 1 && ks == 0 ? 0u : 1u);
       mma_commit(o_full);
       mma_commit(kv_free0 + 8 * stg);
     }
@@ -650,7 +658,7 @@ pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_k
   // few tiles share their positions out among clusters, four tiles of them or more to a CTA
   const long long seen = a.window > 0 ? std::min<long long>(max_context, (long long)a.window + a.n_rows) : max_context;
   int splits = 1;
-  while (splits < 8 && full * a.kv_heads * splits * 2 <= ctx->sm_count && seen / kTileP >= 4 * splits * 2) splits *= 2;
+  while (splits < 8 && full * a.kv_heads * splits * 2 <= ctx->sm_count && seen / 64 >= 8 * splits * 2) splits *= 2;
   const dim3 grid((unsigned)(a.kv_heads * splits), (unsigned)most);
   const bool two = a.dtype == PI_F32;
   if (pool->kind == PI_INT8) {
