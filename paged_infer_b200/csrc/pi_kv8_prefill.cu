@@ -321,8 +321,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const Group* group = s_group[j % STAGES];
       constexpr int COLS = TILE / 2, GROUPS = COLS / 16;   // of this thread
       const uint32_t s_col = lane_addr + L::col_s + buf * TILE + half * COLS;
-      // what the row sees of this thread's groups: their columns first .. last; r goes by all
-      int first[GROUPS], last[GROUPS], v_top = kNoScale;
+      // what the row sees of this thread's groups: a bit per column; r goes by all
+      uint32_t seen[GROUPS];
+      int v_top = kNoScale;
       bool inside = true;
 #pragma unroll
       for (int g = 0; g < 2 * GROUPS; ++g) {
@@ -330,8 +331,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         const int f = max(0, from - q.base), l = min(to - q.base, q.valid - 1);
         if (f <= l) v_top = max(v_top, q.v_exp);
         if (g / GROUPS == half) {
-          first[g % GROUPS] = f;
-          last[g % GROUPS] = l;
+          seen[g % GROUPS] = f <= l ? (0xffffu >> (15 - l)) & (0xffffu << f) : 0;
           inside = inside && f == 0 && l == 15;
         }
       }
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (i < first[g] || i > last[g]) w[g * 16 + i] = -INFINITY;   // times the scale of K: still so, or not a number where that is none
+            if (!(seen[g] & 1u << i)) w[g * 16 + i] = -INFINITY;
       }
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
@@ -386,13 +386,13 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[g * 16 + i] = exp2_fast(fmaf(w[g * 16 + i], f, less));
-        if (masks) {
+        if (masks && !(f > 0.f && f < INFINITY)) {   // minus infinity times this is not minus infinity
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[g * 16 + i] = i >= first[g] && i <= last[g] ? w[g * 16 + i] : 0.f;
+          for (int i = 0; i < 16; ++i) w[g * 16 + i] = seen[g] & 1u << i ? w[g * 16 + i] : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i & 1] += w[g * 16 + i];
-        if (!masks || first[g] <= last[g]) sum = fmaf(part[0] + part[1], exp2_fast(-shift), sum);
+        if (!masks || seen[g]) sum = fmaf(part[0] + part[1], exp2_fast(-shift), sum);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           hi[g * 8 + i] = pack_f16(w[g * 16 + 2 * i], w[g * 16 + 2 * i + 1]);
