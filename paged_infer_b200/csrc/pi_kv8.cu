@@ -7,8 +7,12 @@
 // first token on starts without a past.  All of it is IEEE f32 (1 / top as a constant, one product, one division, one rounding a code), so that codes do
 // not depend on how the rows were dealt to warps.
 //
-// A warp takes a unit's one head and side: four channels a lane, the rows' magnitudes first, then the codes; the second reading
-// comes from the caches.  Nothing is shared between warps.
+// A warp takes a unit's one head and side, four neighbouring channels a lane, several rows at once where a row needs fewer lanes: the
+// rows of a unit of up to 16 (8 for wide heads) are loaded together and stay in registers from their magnitudes to their codes;
+// longer units are read twice.  Nothing is shared between warps.
+//
+// The quotient: q = x r with r = RN(1 / s), and one correction by the remainder, which is RN(x / s) by Markstein's theorem while
+// nothing leaves the normal range; scales at its edges take the division itself.
 #include <math.h>
 
 #include <algorithm>
@@ -28,33 +32,13 @@ struct WriteParams {
   uint8_t* codes;            // of the layer
   float* scales;
   int num_blocks, block_size, kv_heads, head_dim, pitch;
+  pi_divisor by_block;
   const int64_t* slots;
-  int n_rows, rows_per_warp;
+  int n_rows, rows_per_warp;   // a warp looks for units that begin in this many rows, at most 16
 };
 
-// Channels d .. d + 3 of the vector at element `at`, zeros behind the last.
-__device__ __forceinline__ float4 load4(const WriteParams& p, const void* base, size_t at, int d) {
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (d >= p.head_dim) return x;
-  if (p.wide) {
-    if (p.dtype == PI_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + d);
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at + d);
-    if (p.dtype == PI_BF16)
-      return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-  }
-  x.x = pi_load_as_f32(base, at + d, p.dtype);
-  if (d + 1 < p.head_dim) x.y = pi_load_as_f32(base, at + d + 1, p.dtype);
-  if (d + 2 < p.head_dim) x.z = pi_load_as_f32(base, at + d + 2, p.dtype);
-  if (d + 3 < p.head_dim) x.w = pi_load_as_f32(base, at + d + 3, p.dtype);
-  return x;
-}
-
 template <int KIND>
-__device__ __forceinline__ uint32_t encode(float x, float s) {
-  if (!(s > 0.f)) return 0;   // an empty block, or one whose values are not finite
-  const float y = __fdiv_rn(x, s);
+__device__ __forceinline__ uint32_t encode(float y) {   // any quotient
   if (KIND == PI_E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)(int)fminf(fmaxf(roundf(y), -127.f), 127.f) & 0xffu;
 }
@@ -63,14 +47,35 @@ __device__ __forceinline__ float decode(uint32_t code) {
   if (KIND == PI_E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
   return (float)(int8_t)code;
 }
+// Four codes under a scale; r = RN(1 / s) where s is in the middle of the normal range, 0 elsewhere.
 template <int KIND>
-__device__ __forceinline__ uint32_t encode4(float4 x, float s) {
-  return encode<KIND>(x.x, s) | encode<KIND>(x.y, s) << 8 | encode<KIND>(x.z, s) << 16 | encode<KIND>(x.w, s) << 24;
+__device__ __forceinline__ uint32_t encode4(const float* x, float s, float r) {
+  if (r == 0.f) {
+    if (!(s > 0.f)) return 0;   // an empty block, or one whose values are not finite
+    return encode<KIND>(__fdiv_rn(x[0], s)) | encode<KIND>(__fdiv_rn(x[1], s)) << 8 | encode<KIND>(__fdiv_rn(x[2], s)) << 16 | encode<KIND>(__fdiv_rn(x[3], s)) << 24;
+  }
+  float y[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const float q = __fmul_rn(x[b], r);
+    y[b] = __fmaf_rn(__fmaf_rn(-q, s, x[b]), r, q);
+    if (KIND == PI_E4M3 && x[b] == 0.f) y[b] = x[b];   // the remainder has lost the sign of -0, which e4m3 has
+  }
+  if (KIND == PI_E4M3)
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+  // halves away from zero: |y| < 127.5, and the number below 1/2 added to a half makes the next whole one, to less than a half does not
+  uint32_t c[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) c[b] = (uint32_t)(int)(y[b] + copysignf(0.49999997f, y[b]));
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
-template <int KIND>
+// LANES of them to a row, GROUPS of four channels a lane.
+template <int KIND, int LANES, int GROUPS>
 __global__ void __launch_bounds__(kWriteWarps * 32) kv8_write_kernel(const WriteParams p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bs = p.block_size;
+  constexpr int AT_ONCE = 32 / LANES, MOST = GROUPS == 1 ? 16 : 8, STEPS = MOST / AT_ONCE;   // rows at once, rows in registers
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bs = p.block_size, sub = lane / LANES, d0 = 4 * (lane % LANES);
   const long long job = (long long)blockIdx.x * kWriteWarps + warp;
   const int per_row = p.kv_heads * 2, hs = (int)(job % per_row), head = hs >> 1, side = hs & 1;
   const long long row0 = job / per_row * p.rows_per_warp;
@@ -78,67 +83,102 @@ __global__ void __launch_bounds__(kWriteWarps * 32) kv8_write_kernel(const Write
   if (row0 >= p.n_rows) return;
   const void* src = side ? p.v : p.k;
   const size_t stride = side ? p.v_stride : p.k_stride, col = (size_t)head * p.head_dim;
-  const long long row_end = min(row0 + p.rows_per_warp, (long long)p.n_rows);
 
-  long long before = row0 > 0 ? p.slots[row0 - 1] : -1;
-  if (before >= 0) before /= bs;
-  for (long long r = row0; r < row_end;) {
-    const long long slot = p.slots[r], block = slot >= 0 ? slot / bs : -1;
-    if (block < 0 || block >= p.num_blocks || block == before) {   // unmapped, or a unit that began further up
-      before = block;
-      ++r;
-      continue;
+  // lane l looks at row row0 - 1 + l: its block, -1 where it has none
+  auto block_of = [&](long long row) -> int {
+    if (row < 0 || row >= p.n_rows) return -1;
+    const long long slot = p.slots[row];
+    if (slot < 0) return -1;
+    const long long b = slot < 0x7fffffffll ? p.by_block((int)slot) : slot / bs;
+    return b < p.num_blocks ? (int)b : -1;
+  };
+  const int mine = block_of(row0 - 1 + lane), before = __shfl_up_sync(0xffffffffu, mine, 1);
+  unsigned leaders = __ballot_sync(0xffffffffu, lane >= 1 && lane <= p.rows_per_warp && mine >= 0 && mine != before);
+  for (; leaders; leaders &= leaders - 1) {
+    const int l0 = __ffs(leaders) - 1, block = __shfl_sync(0xffffffffu, mine, l0);
+    const long long r = row0 - 1 + l0;
+    // the unit: rows r .. r + n - 1, all in this block
+    const unsigned out = __ballot_sync(0xffffffffu, lane > l0 && mine != block);
+    long long n = (out ? __ffs(out) - 1 : 32) - l0;
+    while (!out) {
+      const unsigned more = __ballot_sync(0xffffffffu, block_of(r + n + lane) != block);
+      n += more ? __ffs(more) - 1 : 32;
+      if (more) break;
     }
-    // the unit: rows r .. end - 1, all in this block
-    long long end = r + 1;
-    while (true) {
-      const long long i = end + lane;
-      const long long there = i < p.n_rows ? p.slots[i] : -1;
-      const unsigned out = __ballot_sync(0xffffffffu, there < block * bs || there >= (block + 1) * bs);
-      if (out) {
-        end += __ffs(out) - 1;
-        break;
-      }
-      end += 32;
-    }
-    const int first = (int)(slot - block * bs);
+    const int first = (int)(p.slots[r] - (long long)block * bs);
+    const size_t tile = ((size_t)block * p.kv_heads + head) * 2 + side;
+    uint8_t* codes = p.codes + tile * (size_t)bs * p.pitch;
+    const float old = first > 0 ? p.scales[tile] : 0.f;
+    float x[STEPS][GROUPS][4];
+    auto load = [&](long long from) {   // up to MOST rows of the unit
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const long long at = from + i * AT_ONCE + sub;
+          const int d = d0 + g * 4 * LANES;
+          pi_load4_as_f32(x[i][g], src, (size_t)(r + at) * stride + col + d, p.dtype, at < n ? p.head_dim - d : 0, p.wide);
+        }
+    };
     float most = 0.f;
     bool odd = false;   // an infinity or NaN: the block's scale says so, whatever comes later
-    for (int d = 4 * lane; d < p.pitch; d += 128)
-#pragma unroll 4
-      for (long long i = r; i < end; ++i) {
-        const float4 x = load4(p, src, (size_t)i * stride + col, d);
-        const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-        odd |= !(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY && fabsf(x.z) < INFINITY && fabsf(x.w) < INFINITY);
-        most = fmaxf(most, m);
-      }
+    for (long long from = 0; from < n; from += MOST) {
+      load(from);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            odd |= !(fabsf(x[i][g][b]) < INFINITY);
+            most = fmaxf(most, fabsf(x[i][g][b]));
+          }
+    }
     most = pi_warp_max(most);
     odd = __any_sync(0xffffffffu, odd);
-    const size_t tile = ((size_t)block * p.kv_heads + head) * 2 + side;
-    const float old = first > 0 ? p.scales[tile] : 0.f;
     float s = fmaxf(old, __fmul_rn(most, KIND == PI_E4M3 ? 1.f / 448.f : 1.f / 127.f));
     if (odd || old != old) s = __int_as_float(0x7fffffff);
-    uint8_t* codes = p.codes + tile * (size_t)bs * p.pitch;
-    if (s != old && s == s && first > 0)
-      for (int d = 4 * lane; d < p.pitch; d += 128)
-#pragma unroll 4
-        for (int t = 0; t < first; ++t) {
+    const float recip = s > 1e-30f && s < 1e30f ? __frcp_rn(s) : 0.f;
+    if (s != old && s == s && first > 0)   // the tokens in front, in the larger scale
+      for (int t = sub; t < first; t += AT_ONCE)
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int d = d0 + g * 4 * LANES;
+          if (d >= p.pitch) continue;
           uint32_t* w = reinterpret_cast<uint32_t*>(codes + (size_t)t * p.pitch + d);
           const uint32_t c = *w;
-          *w = encode4<KIND>(make_float4(__fmul_rn(decode<KIND>(c & 0xff), old), __fmul_rn(decode<KIND>(c >> 8 & 0xff), old), __fmul_rn(decode<KIND>(c >> 16 & 0xff), old),
-                                         __fmul_rn(decode<KIND>(c >> 24), old)), s);
+          const float y[4] = {__fmul_rn(decode<KIND>(c & 0xff), old), __fmul_rn(decode<KIND>(c >> 8 & 0xff), old), __fmul_rn(decode<KIND>(c >> 16 & 0xff), old),
+                              __fmul_rn(decode<KIND>(c >> 24), old)};
+          *w = encode4<KIND>(y, s, recip);
         }
-    for (int d = 4 * lane; d < p.pitch; d += 128)
-#pragma unroll 4
-      for (long long i = r; i < end; ++i) {
-        const int off = (int)(p.slots[i] - block * bs);
-        *reinterpret_cast<uint32_t*>(codes + (size_t)off * p.pitch + d) = encode4<KIND>(load4(p, src, (size_t)i * stride + col, d), s);
-      }
     __syncwarp();
+    for (long long from = 0; from < n; from += MOST) {
+      if (n > MOST) load(from);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const long long at = from + i * AT_ONCE + sub;
+        if (at < n) {
+          const int off = (int)(p.slots[r + at] - (long long)block * bs);
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            const int d = d0 + g * 4 * LANES;
+            if (d < p.pitch) *reinterpret_cast<uint32_t*>(codes + (size_t)off * p.pitch + d) = encode4<KIND>(x[i][g], s, recip);
+          }
+        }
+      }
+      __syncwarp();
+    }
     if (lane == 0) p.scales[tile] = s;
-    before = block;
-    r = end;
   }
+}
+
+template <int KIND>
+cudaError_t launch_write(pi_ctx* ctx, const WriteParams& p, unsigned grid) {
+  const dim3 g(grid), b(kWriteWarps * 32);
+  if (p.pitch == 32) return pi_launch_chained(ctx, kv8_write_kernel<KIND, 8, 1>, g, b, 0, 1, p);
+  if (p.pitch == 64) return pi_launch_chained(ctx, kv8_write_kernel<KIND, 16, 1>, g, b, 0, 1, p);
+  if (p.pitch <= 128) return pi_launch_chained(ctx, kv8_write_kernel<KIND, 32, 1>, g, b, 0, 1, p);
+  return pi_launch_chained(ctx, kv8_write_kernel<KIND, 32, 2>, g, b, 0, 1, p);
 }
 
 }  // namespace
@@ -259,6 +299,7 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
   p.kv_heads = L.num_kv_heads;
   p.head_dim = L.head_dim;
   p.pitch = pool->pitch;
+  p.by_block = pi_divisor(L.block_size);
   p.slots = slots_dev;
   p.n_rows = n_rows;
   // a warp looks for units that begin in this many rows: one while that leaves the GPU room, more for prompts, where most rows begin none
@@ -267,7 +308,7 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
   const long long grid = (jobs + kWriteWarps - 1) / kWriteWarps;
   PI_REQUIRE(ctx, grid <= 0x7fffffffll, "too many rows");
   pi_prof_scope prof(ctx, PI_PROF_ROPE_KV);
-  PI_CUDA(ctx, pi_launch_chained(ctx, pool->kind == PI_E4M3 ? kv8_write_kernel<PI_E4M3> : kv8_write_kernel<PI_INT8>, dim3((unsigned)grid), dim3(kWriteWarps * 32), 0, 1, p));
+  PI_CUDA(ctx, pool->kind == PI_E4M3 ? launch_write<PI_E4M3>(ctx, p, (unsigned)grid) : launch_write<PI_INT8>(ctx, p, (unsigned)grid));
   PI_CHECK_LAUNCH(ctx);
   return PI_OK;
 }
