@@ -85,14 +85,17 @@ __global__ void __launch_bounds__(kWriteWarps * 32) kv8_write_kernel(const Write
   const size_t stride = side ? p.v_stride : p.k_stride, col = (size_t)head * p.head_dim;
 
   // lane l looks at row row0 - 1 + l: its block, -1 where it has none
-  auto block_of = [&](long long row) -> int {
+  auto place_of = [&](long long row, int& off) -> int {
+    off = 0;
     if (row < 0 || row >= p.n_rows) return -1;
     const long long slot = p.slots[row];
     if (slot < 0) return -1;
     const long long b = slot < 0x7fffffffll ? p.by_block((int)slot) : slot / bs;
+    off = (int)(slot - b * bs);
     return b < p.num_blocks ? (int)b : -1;
   };
-  const int mine = block_of(row0 - 1 + lane), before = __shfl_up_sync(0xffffffffu, mine, 1);
+  int my_off, other;
+  const int mine = place_of(row0 - 1 + lane, my_off), before = __shfl_up_sync(0xffffffffu, mine, 1);
   unsigned leaders = __ballot_sync(0xffffffffu, lane >= 1 && lane <= p.rows_per_warp && mine >= 0 && mine != before);
   for (; leaders; leaders &= leaders - 1) {
     const int l0 = __ffs(leaders) - 1, block = __shfl_sync(0xffffffffu, mine, l0);
@@ -101,24 +104,66 @@ __global__ void __launch_bounds__(kWriteWarps * 32) kv8_write_kernel(const Write
     const unsigned out = __ballot_sync(0xffffffffu, lane > l0 && mine != block);
     long long n = (out ? __ffs(out) - 1 : 32) - l0;
     while (!out) {
-      const unsigned more = __ballot_sync(0xffffffffu, block_of(r + n + lane) != block);
+      const unsigned more = __ballot_sync(0xffffffffu, place_of(r + n + lane, other) != block);
       n += more ? __ffs(more) - 1 : 32;
       if (more) break;
     }
-    const int first = (int)(p.slots[r] - (long long)block * bs);
+    const int first = __shfl_sync(0xffffffffu, my_off, l0);
     const size_t tile = ((size_t)block * p.kv_heads + head) * 2 + side;
     uint8_t* codes = p.codes + tile * (size_t)bs * p.pitch;
     const float old = first > 0 ? p.scales[tile] : 0.f;
     float x[STEPS][GROUPS][4];
-    auto load = [&](long long from) {   // up to MOST rows of the unit
+    const size_t start = (size_t)r * stride + col;
+    auto load = [&](long long from) {   // up to MOST rows of the unit, their loads under way together
+      if (p.wide && p.dtype == PI_F32) {
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i)
+        for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
+          for (int g = 0; g < GROUPS; ++g) {
+            const long long at = from + i * AT_ONCE + sub;
+            const int d = d0 + g * 4 * LANES;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at < n && d < p.head_dim) v = *reinterpret_cast<const float4*>(static_cast<const float*>(src) + start + (size_t)at * stride + d);
+            x[i][g][0] = v.x, x[i][g][1] = v.y, x[i][g][2] = v.z, x[i][g][3] = v.w;
+          }
+      } else if (p.wide) {
+        uint2 raw[STEPS][GROUPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            const long long at = from + i * AT_ONCE + sub;
+            const int d = d0 + g * 4 * LANES;
+            raw[i][g] = make_uint2(0, 0);
+            if (at < n && d < p.head_dim) raw[i][g] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(src) + start + (size_t)at * stride + d);
+          }
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            const uint2 w = raw[i][g];
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+            const bool bf = p.dtype == PI_BF16;
+            x[i][g][0] = bf ? __uint_as_float(w.x << 16) : a.x, x[i][g][1] = bf ? __uint_as_float(w.x & 0xffff0000u) : a.y;
+            x[i][g][2] = bf ? __uint_as_float(w.y << 16) : b.x, x[i][g][3] = bf ? __uint_as_float(w.y & 0xffff0000u) : b.y;
+          }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < STEPS; ++i) {
           const long long at = from + i * AT_ONCE + sub;
-          const int d = d0 + g * 4 * LANES;
-          pi_load4_as_f32(x[i][g], src, (size_t)(r + at) * stride + col + d, p.dtype, at < n ? p.head_dim - d : 0, p.wide);
+          float y[GROUPS][4];
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) pi_load4_as_f32(y[g], src, start + (size_t)at * stride + d0 + g * 4 * LANES, p.dtype, at < n ? p.head_dim - d0 - g * 4 * LANES : 0, false);
+#pragma unroll
+          for (int e = 0; e < STEPS; ++e)
+            if (e == i) {
+#pragma unroll
+              for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) x[e][g][b] = y[g][b];
+            }
         }
+      }
     };
     float most = 0.f;
     bool odd = false;   // an infinity or NaN: the block's scale says so, whatever comes later
@@ -157,8 +202,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32) kv8_write_kernel(const Write
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const long long at = from + i * AT_ONCE + sub;
+        int off = __shfl_sync(0xffffffffu, my_off, (int)min(l0 + at, 31ll));
         if (at < n) {
-          const int off = (int)(p.slots[r + at] - (long long)block * bs);
+          if (l0 + at > 31) off = (int)(p.slots[r + at] - (long long)block * bs);
 #pragma unroll
           for (int g = 0; g < GROUPS; ++g) {
             const int d = d0 + g * 4 * LANES;
