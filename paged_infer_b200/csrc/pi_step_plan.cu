@@ -13,12 +13,13 @@
 
 namespace {
 
-constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32, kPlanMaxSeqs = 16384;
+constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32, kPlanMaxSeqs = 16384;   // at most
 
 struct PlanParams {
   pi_step_arrays a;
   const int32_t *start, *n_tokens, *free_list;
   int n_seqs, n_free;
+  pi_divisor by_block;
 };
 
 struct Totals {
@@ -29,7 +30,8 @@ __device__ __forceinline__ void plan_sequence(const PlanParams& p, int b, int& s
   const int bs = p.a.block_size, wide = p.a.max_blocks;
   start = max(p.start[b], 0);
   n = max(p.n_tokens[b], 0);
-  const long long held_all = ((long long)start + bs - 1) / bs, after_all = ((long long)start + n + bs - 1) / bs;
+  const long long end = (long long)start + n + bs - 1;
+  const long long held_all = end < 0x7fffffffll ? p.by_block(start + bs - 1) : ((long long)start + bs - 1) / bs, after_all = end < 0x7fffffffll ? p.by_block((int)end) : end / bs;
   held = (int)min(held_all, (long long)wide);
   after = (int)min(after_all, (long long)wide);
   spill = after_all - max(held_all, (long long)after);   // blocks that the table's row has no room for
@@ -37,13 +39,13 @@ __device__ __forceinline__ void plan_sequence(const PlanParams& p, int b, int& s
 
 __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const PlanParams p) {
   extern __shared__ int s_plan[];
-  const int B = p.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = p.a.block_size, wide = p.a.max_blocks;
+  const int B = p.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5, bs = p.a.block_size, wide = p.a.max_blocks;
   int *s_cu = s_plan, *s_free = s_cu + B + 1, *s_start = s_free + B;   // first row, first entry of the free list, start
   __shared__ Totals s_warp[kPlanWarps];
   pi_grid_dependency_wait();
 
   // prefix sums: a run of sequences per thread, a scan of the runs' totals
-  const int per = (B + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, B), b1 = min(b0 + per, B);
+  const int per = (B + threads - 1) / threads, b0 = min(tid * per, B), b1 = min(b0 + per, B);
   Totals mine = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
     int start, held, after;
@@ -56,26 +58,39 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const PlanParam
   Totals upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long r = __shfl_up_sync(0xffffffffu, upto.rows, o), f = __shfl_up_sync(0xffffffffu, upto.need, o), s = __shfl_up_sync(0xffffffffu, upto.spill, o);
+    const long long r = __shfl_up_sync(0xffffffffu, upto.rows, o), f = __shfl_up_sync(0xffffffffu, upto.need, o);
     if (lane >= o) {
       upto.rows += r;
       upto.need += f;
-      upto.spill += s;
     }
+  }
+  if (__any_sync(0xffffffffu, mine.spill != 0)) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) upto.spill += __shfl_xor_sync(0xffffffffu, upto.spill, o);
   }
   if (lane == 31) s_warp[warp] = upto;
   __syncthreads();
-  Totals ahead = {upto.rows - mine.rows, upto.need - mine.need, 0}, total = {0, 0, 0};
-  for (int w = 0; w < kPlanWarps; ++w) {
-    const Totals t = s_warp[w];
-    if (w < warp) {
-      ahead.rows += t.rows;
-      ahead.need += t.need;
-    }
-    total.rows += t.rows;
-    total.need += t.need;
-    total.spill += t.spill;
+  // lane w looks at warp w
+  Totals ahead = lane < warps ? s_warp[lane] : Totals{0, 0, 0}, total = ahead;
+  if (lane >= warp) ahead.rows = ahead.need = 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o >= warps) continue;   // further lanes hold nothing
+    ahead.rows += __shfl_xor_sync(0xffffffffu, ahead.rows, o);
+    ahead.need += __shfl_xor_sync(0xffffffffu, ahead.need, o);
+    total.rows += __shfl_xor_sync(0xffffffffu, total.rows, o);
+    total.need += __shfl_xor_sync(0xffffffffu, total.need, o);
+    total.spill += __shfl_xor_sync(0xffffffffu, total.spill, o);
   }
+  if (warps < 32) {
+    ahead.rows = __shfl_sync(0xffffffffu, ahead.rows, 0);
+    ahead.need = __shfl_sync(0xffffffffu, ahead.need, 0);
+    total.rows = __shfl_sync(0xffffffffu, total.rows, 0);
+    total.need = __shfl_sync(0xffffffffu, total.need, 0);
+    total.spill = __shfl_sync(0xffffffffu, total.spill, 0);
+  }
+  ahead.rows += upto.rows - mine.rows;
+  ahead.need += upto.need - mine.need;
   const long long cap = p.a.max_rows;
   for (int b = b0; b < b1; ++b) {
     int start, held, after;
@@ -104,7 +119,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const PlanParam
   __syncthreads();
 
   // new table entries: a warp per sequence
-  for (int b = blockIdx.x * kPlanWarps + warp; b < B; b += gridDim.x * kPlanWarps) {
+  for (int b = blockIdx.x * warps + warp; b < B; b += gridDim.x * warps) {
     int start, held, after;
     long long n, spill;
     plan_sequence(p, b, start, n, held, after, spill);
@@ -114,7 +129,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const PlanParam
     }
   }
   // rows: entries below `held` are read from the table, the ones above from where they come from
-  for (long long r = (long long)blockIdx.x * kPlanThreads + tid; r < cap; r += (long long)gridDim.x * kPlanThreads) {
+  for (long long r = (long long)blockIdx.x * threads + tid; r < cap; r += (long long)gridDim.x * threads) {
     int seq = -1, pos = -1;
     long long slot = -1;
     if (r < s_cu[B]) {
@@ -126,8 +141,9 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const PlanParam
       }
       seq = lo;
       const long long at = (long long)s_start[seq] + (r - s_cu[seq]);
-      const long long lb = at / bs;
-      const int held = (int)min(((long long)s_start[seq] + bs - 1) / bs, (long long)wide);
+      const long long lb = at < 0x7fffffffll ? p.by_block((int)at) : at / bs;
+      const long long before = (long long)s_start[seq] + bs - 1;
+      const int held = (int)min(before < 0x7fffffffll ? (long long)p.by_block((int)before) : before / bs, (long long)wide);
       pos = (int)at;
       int block = -1;
       if (lb < held) block = p.a.tables[(size_t)seq * wide + lb];
@@ -156,10 +172,12 @@ extern "C" pi_status pi_step_plan(pi_ctx* ctx, const pi_step_arrays* a, const in
     PI_CUDA(ctx, cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     grant.of(ctx) = most;
   }
-  const long long shares = std::max<long long>({1, ((long long)a->max_rows + kPlanThreads - 1) / kPlanThreads, ((long long)n_seqs + kPlanWarps - 1) / kPlanWarps});
+  // as many threads as there are rows or sequences, up to a whole CTA; more CTAs for more rows than that
+  const int busy = std::max(n_seqs, std::min(a->max_rows, kPlanThreads)), threads = std::min(kPlanThreads, (busy + 31) / 32 * 32), warps = threads / 32;
+  const long long shares = std::max<long long>({1, ((long long)a->max_rows + threads - 1) / threads, ((long long)n_seqs + warps - 1) / warps});
   pi_prof_scope prof(ctx, PI_PROF_OTHER);
-  const PlanParams p = {*a, start_dev, n_tokens_dev, free_dev, n_seqs, n_free};
-  PI_CUDA(ctx, pi_launch_chained(ctx, step_plan_kernel, dim3((unsigned)std::min<long long>(shares, ctx->sm_count)), dim3(kPlanThreads), smem, 1, p));
+  const PlanParams p = {*a, start_dev, n_tokens_dev, free_dev, n_seqs, n_free, pi_divisor(a->block_size)};
+  PI_CUDA(ctx, pi_launch_chained(ctx, step_plan_kernel, dim3((unsigned)std::min<long long>(shares, ctx->sm_count)), dim3(threads), smem, 1, p));
   PI_CHECK_LAUNCH(ctx);
   return PI_OK;
 }
