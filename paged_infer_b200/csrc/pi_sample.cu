@@ -29,7 +29,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2 * kThreads, kBinBits = 10, kMaxCluster = 8;   // two bins per thread
 constexpr int kWeightBits = 45, kLimb = 15;
 constexpr int kSliceFloats = 48 * 1024;   // logits that fit a CTA's shared memory beside the histograms
-constexpr int kTable = 32;                // floats that 16 doubles take
+constexpr int kTable = 64;                // floats that 32 doubles take
 
 struct SampleParams {
   const void* logits;
@@ -89,34 +89,40 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
   return v;
 }
 
-// 2^(j / 16), and ln(2)^k / k!
-__device__ const double kRoots[16] = {1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
-                                      1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+// 2^(j / 32)
+__device__ const double kRoots[32] = {1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+                                      1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+                                      1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+                                      1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+                                      1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
+                                      1.9152065613971474, 1.9571441241754002};
 
 struct Row {
   const float* x;       // the slice
   int count;
   float most, scale;    // bins per unit of logit
-  double rate;          // log2(e) / T
-  // 2^y for y = (v - most) rate <= 0: a sixteenth from the table, the rest g, |g| <= 1/32, by its series up to g^6 (the next term is below
-  // 2^-51), as a multiple of 2^-45
+  double rate, offset;  // log2(e) / T, and minus that times `most`
+  // 2^y for y = (v - most) rate <= 0: a 32nd from the table, the rest g, |g| <= 1/64, by its series up to g^5 (the next term is below 2^-48),
+  // as a multiple of 2^-45
   __device__ __forceinline__ unsigned long long weight(float v) const {
     extern __shared__ __align__(16) float s_slice[];
     if (v == most) return 1ull << kWeightBits;
-    const double y = ((double)v - (double)most) * rate;
+    // f32 to f64 by its bits; what is below the normal range counts as 0
+    const uint32_t bits = __float_as_uint(v), mag = bits & 0x7fffffffu;
+    const double wide = mag < 0x00800000u ? 0.0 : __hiloint2double((int)((bits & 0x80000000u) | ((mag >> 3) + (896u << 20))), (int)(bits << 29));
+    const double y = fma(wide, rate, offset);
     if (!(y > -60.0)) return 0;
-    const double shifted = y + 422212465065984.0;                  // 1.5 2^48: the low bits of the sum count sixteenths
+    const double shifted = y + 211106232532992.0;                  // 1.5 2^47: the low bits of the sum count 32nds
     const int k = __double2loint(shifted);
-    const double g = y - (shifted - 422212465065984.0);
-    double e = 1.5403530393381608e-4;                              // ln(2)^6 / 6!
-    e = fma(e, g, 1.3333558146428443e-3);
+    const double g = y - (shifted - 211106232532992.0);
+    double e = 1.3333558146428441e-3;                              // ln(2)^5 / 5!
     e = fma(e, g, 9.618129107628477e-3);
-    e = fma(e, g, 5.550410866482158e-2);
+    e = fma(e, g, 5.5504108664821576e-2);
     e = fma(e, g, 2.402265069591007e-1);
     e = fma(e, g, 6.931471805599453e-1);
-    const double root = reinterpret_cast<const double*>(s_slice)[k & 15];   // the table lies in front of the slice
+    const double root = reinterpret_cast<const double*>(s_slice)[k & 31];   // the table lies in front of the slice
     e = fma(e * g, root, root);
-    const int n = (k >> 4) + kWeightBits;                          // times 2^n, n >= -15
+    const int n = (k >> 5) + kWeightBits;                          // times 2^n, n >= -15
     const double w = __hiloint2double(__double2hiint(e) + (n << 20), __double2loint(e)) + 4503599627370496.0;   // 2^52: rounds to a whole number
     return (unsigned long long)__double_as_longlong(w) & 0xfffffffffffffull;
   }
@@ -145,12 +151,16 @@ __device__ __forceinline__ T scan(T v, T* s_warp, T& all) {
   }
   if (lane == 31) s_warp[warp] = v;
   __syncthreads();
-  all = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    const T t = s_warp[w];
-    if (w < warp) v += t;
-    all += t;
+  T t = s_warp[lane & (kWarps - 1)];   // lanes 16 and up hold the same again
+  T upto = t;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const T u = __shfl_up_sync(0xffffffffu, upto, o, kWarps);
+    if ((lane & (kWarps - 1)) >= o) upto += u;
   }
+  all = __shfl_sync(0xffffffffu, upto, kWarps - 1);
+  const T before = __shfl_sync(0xffffffffu, upto - t, warp);
+  v += before;
   __syncthreads();
   return v;
 }
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int from = min((int)rank * p.per, p.n), count = min(p.per, p.n - from);
   const size_t base = (size_t)r * p.stride + from;
   float* const slice = s_slice + kTable + 6 * kBins / ranks;
-  if (tid < 16) reinterpret_cast<double*>(s_slice)[tid] = kRoots[tid];
+  if (tid < 32) reinterpret_cast<double*>(s_slice)[tid] = kRoots[tid];
   pi_grid_dependency_wait();
 
   // the slice, and the largest logit; NaN counts as minus infinity, -0 as 0
@@ -272,10 +282,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   s.hist[0][tid] = s.hist[0][tid + kThreads] = 0;
   if (2 * tid < kBins / ranks) home_bins()[2 * tid] = home_bins()[2 * tid + 1] = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) best = fmaxf(best, s.warp_f[w]);
-    s.shown.most = ordered(best);
-    s.shown.at = 0x7fffffff;
+  if (warp == 0) {
+    best = pi_warp_max(s.warp_f[lane & (kWarps - 1)]);
+    if (lane == 0) {
+      s.shown.most = ordered(best);
+      s.shown.at = 0x7fffffff;
+    }
   }
   cluster_sync();
   const uint32_t high = __reduce_max_sync(0xffffffffu, lane < ranks ? peer(&s.shown.most, lane) : 0);
@@ -301,7 +313,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const float min_p = p.min_p[r];
   if (min_p > 0.f) exact_bound = max(exact_bound, (double)most + (double)temperature * log(min((double)min_p, 1.0)));
   const float bound = most == INFINITY ? INFINITY : max(__double2float_ru(exact_bound), -FLT_MAX);
-  const Row row = {slice, count, most, (float)kBins / (most - bound), 1.4426950408889634 / (double)temperature};
+  const double rate = 1.4426950408889634 / (double)temperature;
+  // (rates that overflow leave the largest logit alone: everything else weighs 0)
+  const Row row = {slice, count, most, (float)kBins / (most - bound), rate, -(double)most * rate};
 
   const int k = p.top_k[r];
   const float top_p = p.top_p[r];
@@ -400,10 +414,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           s.warp_s[2][warp] = in;
         }
         __syncthreads();
-        if (tid < 3) {
-          unsigned long long t = 0;
-          for (int w = 0; w < kWarps; ++w) t += s.warp_s[tid][w];
-          s.shown.sums[round & 1][tid] = t;
+        if (warp < 3) {
+          const unsigned long long t = warp_sum(lane < kWarps ? s.warp_s[warp][lane] : 0);
+          if (lane == 0) s.shown.sums[round & 1][warp] = t;
         }
         cluster_sync();
         unsigned long long t[3] = {low_weight, low_bin < first ? low_weight : 0, low_bin >= first && low_bin <= last ? low_weight : 0};
@@ -448,15 +461,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     s.warp_b[warp] = same;
   }
   __syncthreads();
-  if (tid == 0) {
-    unsigned long long a = 0;
-    unsigned int b = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      a += s.warp_a[w];
-      b += s.warp_b[w];
+  const unsigned long long in_warp = lane < kWarps ? s.warp_a[lane] : 0;   // lane w looks at warp w
+  const unsigned int equal_in_warp = lane < kWarps ? s.warp_b[lane] : 0;
+  if (warp == 0) {
+    const unsigned long long a = warp_sum(in_warp);
+    const unsigned int b = __reduce_add_sync(0xffffffffu, equal_in_warp);
+    if (lane == 0) {
+      s.shown.weight = a;
+      s.shown.ties = b;
     }
-    s.shown.weight = a;
-    s.shown.ties = b;
   }
   cluster_sync();
   const unsigned long long w_thr = row.weight(from_ordered(thr));
@@ -473,13 +486,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   unsigned long long goal = u > 0.f ? (unsigned long long)floor((double)u * (double)total) : 0;
   goal = min(goal, total - 1);
   // the first token whose running sum exceeds the goal: the warp whose run holds it finds it
-  unsigned long long mine = ahead, taken = used_here;
-  for (int w = 0; w < warp; ++w) {
-    const unsigned long long equal = min((unsigned long long)s.warp_b[w], ties - taken);
-    mine += s.warp_a[w] + equal * w_thr;
-    taken += equal;
+  unsigned int upto_equal = equal_in_warp;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const unsigned int t = __shfl_up_sync(0xffffffffu, upto_equal, o);
+    if (lane >= o) upto_equal += t;
   }
-  const unsigned long long here = s.warp_a[warp] + min((unsigned long long)s.warp_b[warp], ties - taken) * w_thr;
+  const unsigned long long taken_upto = min(used_here + upto_equal, ties), taken_before = min(used_here + (upto_equal - equal_in_warp), ties);
+  const unsigned long long holds = in_warp + (taken_upto - taken_before) * w_thr;
+  unsigned long long holds_upto = holds;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const unsigned long long t = __shfl_up_sync(0xffffffffu, holds_upto, o);
+    if (lane >= o) holds_upto += t;
+  }
+  unsigned long long mine = ahead + __shfl_sync(0xffffffffu, holds_upto - holds, warp), taken = __shfl_sync(0xffffffffu, taken_before, warp);
+  const unsigned long long here = __shfl_sync(0xffffffffu, holds, warp);
   if (goal >= mine && goal < mine + here) {
     for (int i = i0 + lane; i - lane < i1; i += 32) {
       const float x = i < i1 ? slice[i] : -INFINITY;
