@@ -52,6 +52,9 @@ struct Group {
 constexpr int kNoScale = -100000;   // v_exp of a zero scale
 
 __device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A try may suspend the thread for a while that the hardware limits; tries end after kSpinP of them or about a second.  (Polling with
@@ -321,21 +324,30 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const Group* group = s_group[j % STAGES];
       constexpr int COLS = TILE / 2, GROUPS = COLS / 16;   // of this thread
       const uint32_t s_col = lane_addr + L::col_s + buf * TILE + half * COLS;
-      // what the row sees of this thread's groups: a bit per column; r goes by all
+      // the tile as a whole: lane g looks at group g
+      int v_top, lowest, highest;
+      bool filled;
+      {
+        const bool there = lane < 2 * GROUPS;
+        const Group q = group[there ? lane : 0];
+        v_top = __reduce_max_sync(0xffffffffu, there ? q.v_exp : kNoScale);
+        lowest = __reduce_min_sync(0xffffffffu, q.base);
+        highest = __reduce_max_sync(0xffffffffu, q.base + 15);
+        filled = __all_sync(0xffffffffu, q.valid == 16);
+      }
+      const bool masks = !__all_sync(0xffffffffu, filled && from <= lowest && to >= highest);
+      // where not all of it is seen: a bit per column of this thread's groups; r goes by what the row sees
       uint32_t seen[GROUPS];
-      int v_top = kNoScale;
-      bool inside = true;
+      if (masks) {
+        v_top = kNoScale;
 #pragma unroll
-      for (int g = 0; g < 2 * GROUPS; ++g) {
-        const Group q = group[g];
-        const int f = max(0, from - q.base), l = min(to - q.base, q.valid - 1);
-        if (f <= l) v_top = max(v_top, q.v_exp);
-        if (g / GROUPS == half) {
-          seen[g % GROUPS] = f <= l ? (0xffffu >> (15 - l)) & (0xffffu << f) : 0;
-          inside = inside && f == 0 && l == 15;
+        for (int g = 0; g < 2 * GROUPS; ++g) {
+          const Group q = group[g];
+          const int f = max(0, from - q.base), l = min(to - q.base, q.valid - 1);
+          if (f <= l) v_top = max(v_top, q.v_exp);
+          if (g / GROUPS == half) seen[g % GROUPS] = f <= l ? (0xffffu >> (15 - l)) & (0xffffu << f) : 0;
         }
       }
-      const bool masks = !__all_sync(0xffffffffu, inside);
       const int v_unit = v_top == kNoScale ? 0 : min(v_top + 1, 126);   // r = 2^v_unit
       float w[COLS];
       {
@@ -506,8 +518,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         if (lane == 0) fail(23);
         break;
       }
-      unsigned char* kdst = smem + (size_t)stg * L::stage;
-      unsigned char* vdst = kdst + L::side;
+      // addresses of 16-byte chunks: the swizzle is an exclusive or with bits of the row, which are the thread's own
+      const uint32_t kdst = smem_base + stg * L::stage + (part * kPartP + k_token) * 128 + ((k_token & 7) << 4);
+      const uint32_t vdst = smem_base + stg * L::stage + L::side + part * (HD * 128) + v_part * (HD / 16) * 128 + ((v_eight ^ (v_part * (HD / 16) & 7)) << 4);
       if (lane == 0) {   // token 16 cw: this thread's token of K
         Group q;
         q.base = k_here.base;
@@ -525,9 +538,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           const uint32_t a = unsign<KIND>(cur.k[2 * c]), b = unsign<KIND>(cur.k[2 * c + 1]);
-          const uint4 x = make_uint4(widen<KIND, false>(a, false), widen<KIND, false>(a, true), widen<KIND, false>(b, false), widen<KIND, false>(b, true));
           const int chunk = HD == 128 ? c : k_half * CHUNKS + c, sub = HD == 128 ? k_half : 0;
-          *reinterpret_cast<uint4*>(kdst + sub * (TILE * 128) + (part * kPartP + k_token) * 128 + ((chunk ^ (k_token & 7)) << 4)) = x;
+          st_shared((kdst ^ chunk << 4) + sub * (TILE * 128), widen<KIND, false>(a, false), widen<KIND, false>(a, true), widen<KIND, false>(b, false), widen<KIND, false>(b, true));
         }
       }
       {   // V: eight tokens of a channel are 16 bytes, [part][channel][128 bytes] swizzled
@@ -543,9 +555,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
             for (int t = 0; t < 4; ++t) x[t] = __byte_perm(u[2 * t], u[2 * t + 1], half ? 0x7362 : 0x5140);
 #pragma unroll
             for (int one = 0; one < 2; ++one) {
-              const int d = v_part * (HD / 16) + w * 4 + half * 2 + one;
-              const uint4 y = make_uint4(widen<KIND, false>(x[0], one), widen<KIND, false>(x[1], one), widen<KIND, false>(x[2], one), widen<KIND, false>(x[3], one));
-              *reinterpret_cast<uint4*>(vdst + part * (HD * 128) + d * 128 + ((v_eight ^ (d & 7)) << 4)) = y;
+              const int i = w * 4 + half * 2 + one;   // of this thread's channels, which begin at a multiple of their number
+              st_shared((vdst ^ i << 4) + i * 128, widen<KIND, false>(x[0], one), widen<KIND, false>(x[1], one), widen<KIND, false>(x[2], one), widen<KIND, false>(x[3], one));
             }
           }
         }
