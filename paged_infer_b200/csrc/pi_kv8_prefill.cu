@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[g * 16 + i] = exp2_fast(fmaf(w[g * 16 + i], f, less));
-        if (masks && !(f > 0.f && f < INFINITY)) {   // minus infinity times this is not minus infinity
+        if (masks && !(f > 0.f && f < INFINITY && less < INFINITY)) {   // minus infinity times f plus `less` is not minus infinity
 #pragma unroll
           for (int i = 0; i < 16; ++i) w[g * 16 + i] = seen[g] & 1u << i ? w[g * 16 + i] : 0.f;
         }

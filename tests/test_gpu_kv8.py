@@ -287,7 +287,23 @@ def test_attention_of_long_contexts(ctx, dtype, contexts, window):
     attention_case(ctx, "int8", dtype, 16, 8, 2, 64, contexts, [1] * len(contexts), window=window, seed=9)
 
 
-@pytest.mark.parametrize("news", [[1, 1, 1, 1, 1, 1], [20, 1, 3, 40, 1, 1]])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,contexts,news,window", [(8, 1, 64, [3000], [20], 0), (8, 2, 128, [2500, 40], [33, 40], 0), (16, 1, 128, [2100], [9], 1500), (4, 1, 128, [5000], [40], 0),
+                                                                       (96, 1, 64, [300, 1700], [1, 3], 0), (200, 2, 64, [700], [2], 0), (150, 1, 128, [90], [3], 0)])
+def test_attention_of_portions_behind_long_contexts(ctx, dtype, heads, kv_heads, dim, contexts, news, window):
+    """Few tiles of rows, whose positions a cluster shares; groups wider than a product, and than a tile."""
+    attention_case(ctx, "e4m3" if dim == 64 else "int8", dtype, 16, heads, kv_heads, dim, contexts, news, window=window, seed=heads)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_of_many_sequences(ctx, dtype):
+    """More sequences than a warp looks at once, portions, single tokens and nothing among them."""
+    rng = np.random.default_rng(4)
+    news = rng.choice([0, 1, 1, 2, 40, 70], 75)
+    attention_case(ctx, "int8", dtype, 16, 2, 1, 64, news + rng.integers(0, 60, 75), news, seed=4, pad=5)
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1, 1, 1, 1], [20, 1, 3, 40, 1, 1], [90, 16, 3, 100, 31, 64]])
 def test_attention_over_tables_with_holes(ctx, news):
     for dtype in ("f32", "bf16"):
         attention_case(ctx, "int8", dtype, 16, 8, 2, 64, [200, 16, 3, 150, 31, 64], news, seed=11, holes=True)
@@ -304,16 +320,18 @@ def test_attention_without_hints_and_with_wrong_ones(ctx):
 def test_attention_scores_far_apart_and_scales_far_apart(ctx):
     """Sharp weights, and blocks whose scales differ by orders of magnitude."""
     for dtype in ("f32", "bf16"):
-        attention_case(ctx, "int8", dtype, 16, 4, 2, 64, [150, 300], [1, 20], seed=2, scale=3.0)
-        attention_case(ctx, "int8", dtype, 16, 4, 2, 64, [150, 300], [1, 20], seed=2, spread=3.0, q_scale=0.05)
-    attention_case(ctx, "int8", "f32", 16, 4, 2, 64, [60, 90], [1, 10], seed=6, q_scale=1e30, scale=1e-31)
-    attention_case(ctx, "e4m3", "f32", 16, 4, 2, 64, [60, 90], [1, 10], seed=6, q_scale=1e-30, scale=1e29)
+        for news in ([1, 20], [1, 130]):
+            attention_case(ctx, "int8", dtype, 16, 4, 2, 64, [150, 300], news, seed=2, scale=3.0)
+            attention_case(ctx, "int8", dtype, 16, 4, 2, 64, [150, 300], news, seed=2, spread=3.0, q_scale=0.05)
+    for news in ([1, 10], [1, 80]):
+        attention_case(ctx, "int8", "f32", 16, 4, 2, 64, [60, 90], news, seed=6, q_scale=1e30, scale=1e-31)
+        attention_case(ctx, "e4m3", "f32", 16, 4, 2, 64, [60, 90], news, seed=6, q_scale=1e-30, scale=1e29)
 
 
-@pytest.mark.parametrize("news", [[1], [30]])
+@pytest.mark.parametrize("news", [[1], [30], [90]])
 def test_attention_with_values_that_are_not_finite(ctx, news):
     """A block whose scales are NaN reaches the rows that see one of its tokens and no others."""
-    q, out, cache, plan, given = attention_case(ctx, "int8", "f32", 16, 4, 2, 64, [100], news, seed=1, window=40)
+    q, out, cache, plan, given = attention_case(ctx, "int8", "f32", 16, 4, 2, 64, [100], news, seed=1, window=40, hints=False)
     tables, pos = given["tables"], given["pos"]
     for b, side in ((2, 0), (3, 1), (4, 1), (4, 0)):
         keep = cache.scales.clone()
