@@ -59,19 +59,23 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm vol
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A try may suspend the thread for a while that the hardware limits; tries end after kSpinP of them or about a second.  (Polling with
 // test_wait, 700 times a tile and SM, cost a third of the issue slots and made every wait on a barrier 400 clocks long.)
+// Converters, who are ahead, sleep between theirs.
+template <bool NAP = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   const long long until = clock64() + (1ll << 31);
   for (uint32_t spin = 0; spin < kSpinP; ++spin) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
+    if (NAP) __nanosleep(200);
     if (clock64() > until) return false;
   }
   return false;
 }
+template <bool NAP = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int lane) {
   int ok = 1;
-  if (lane == 0) ok = (!*abort_flag && bar_wait(bar, parity)) ? 1 : 0;
+  if (lane == 0) ok = (!*abort_flag && bar_wait<NAP>(bar, parity)) ? 1 : 0;
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 // K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
@@ -489,19 +493,23 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       if ((uint32_t)v_at.id < (uint32_t)p.num_blocks) {
         const unsigned long long id = (uint32_t)v_at.id;
         const uint8_t* v = p.codes + id * p.block_bytes + ((size_t)kvh * 2 + 1) * p.side_bytes + v_part * (HD / 16);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          // tokens that no row sees stay zero: their bytes may be anything, also what e4m3 calls NaN
-          const int off = (v_eight & 1) * 8 + t;
-          if (v_at.sub + off < bs && v_at.base + off >= lo_all && v_at.base + off <= hi_all) {
-            const uint8_t* at = v + (size_t)(v_at.sub + off) * HD;
-            if constexpr (VW == 2) {
-              const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
-              r.v[t][0] = x.x, r.v[t][1] = x.y;
-            } else {
-              r.v[t][0] = __ldcs(reinterpret_cast<const uint32_t*>(at));
-            }
+        const int off0 = (v_eight & 1) * 8;
+        v += (size_t)(v_at.sub + off0) * HD;
+        auto take = [&](int t) {
+          if constexpr (VW == 2) {
+            const uint2 x = __ldcs(reinterpret_cast<const uint2*>(v + t * HD));
+            r.v[t][0] = x.x, r.v[t][1] = x.y;
+          } else {
+            r.v[t][0] = __ldcs(reinterpret_cast<const uint32_t*>(v + t * HD));
           }
+        };
+        if (v_at.sub + 16 <= bs && v_at.base >= lo_all && v_at.base + 15 <= hi_all) {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) take(t);
+        } else {   // tokens that no row sees stay zero: their bytes may be anything, also what e4m3 calls NaN
+#pragma unroll
+          for (int t = 0; t < 8; ++t)
+            if (v_at.sub + off0 + t < bs && v_at.base + off0 + t >= lo_all && v_at.base + off0 + t <= hi_all) take(t);
         }
         r.v_scale = __ldg(p.scales + (id * p.kv_heads + kvh) * 2 + 1);
       }
@@ -514,7 +522,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const int stg = j % STAGES;
       const Place k_next = locate(j + EVERY, k_token >> 4);
       v_here = locate(j + EVERY, v_eight >> 1);
-      if (!warp_wait(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort, lane)) {
+      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort, lane)) {
         if (lane == 0) fail(23);
         break;
       }
