@@ -508,7 +508,8 @@ pi_status pi_model_read_layer(pi_ctx* ctx, const pi_model* model, int layer, int
  * lengths of its requests, its keys and values are stored as 8-bit codes, attention reads those, and its tokens are drawn
  * from logits on the device.  All pointers are device memory on the context's device, all calls are ordered on the
  * context's stream, allocate nothing, wait for nothing on the host and may be captured into a CUDA graph (after a first
- * call of the same kind outside one); none of them keeps scratch memory, so contexts and graphs never share any.
+ * call of the same kind outside one), which then needs the context, the pool and the tensors for as long as it is replayed;
+ * none of them keeps scratch memory, so contexts and graphs never share any.
  * No counterpart in the reference. */
 
 /* The arrays of a step, all the caller's.  Rows are numbered through, sequence by sequence. */
@@ -541,6 +542,7 @@ pi_status pi_step_plan(pi_ctx* ctx, const pi_step_arrays* arrays, const int32_t*
  * [layer][block][kv_head][k|v] f32, value = code * scale.  pitch is head_dim rounded up to 32, 64, 96, 128, 192 or 256
  * bytes; the bytes behind head_dim are written as zeros.  codes_dev (16-byte aligned) and scales_dev (8-byte aligned) are
  * memory of the caller in this layout that outlives the pool, or both NULL: the pool allocates its own, contents undefined.
+ * Scales are not negative; e4m3 codes that stand for NaN are never written, and attention takes them to be none.
  * head_dim <= 256, block_size <= 4096, num_kv_heads <= 1024. */
 pi_status pi_kv8_pool_create(pi_ctx* ctx, const pi_kv_layout* layout, int kind, void* codes_dev_or_null, float* scales_dev_or_null,
                              pi_kv8_pool** out);
@@ -572,7 +574,8 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
  * h / (num_heads / num_kv_heads).  Weights are softmax(scale q k), accumulated in f32.  tables, lens, cu_rows and row_pos
  * of `arrays` are read (the others may be NULL), of its first n_seqs sequences; rows outside every sequence are not written.
  * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut,
- * and with that the order of sums; results are right whatever they say. */
+ * and with that the order of sums; results are right whatever they say.  At most 65535 sequences, and as many tiles of
+ * 128 (row, head) pairs. */
 pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int num_heads, int dtype, const void* q_dev, size_t q_stride,
                            void* out_dev, size_t out_stride, const pi_step_arrays* arrays, int n_seqs, int n_rows, int max_seq_rows,
                            int max_context, int window, float scale);

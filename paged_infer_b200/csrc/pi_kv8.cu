@@ -13,6 +13,9 @@
 //
 // The quotient: q = x r with r = RN(1 / s), and one correction by the remainder, which is RN(x / s) by Markstein's theorem while
 // nothing leaves the normal range; scales at its edges take the division itself.
+//
+// Bound: latency, of the slots, then the rows, then the codes' stores, with 16 warps an SM.  Measured: 4200 rows of 8 heads of 128, bf16
+// to e4m3: 15 us, 1.7 TB/s (31 us with rows read twice and one load at a time).
 #include <math.h>
 
 #include <algorithm>
@@ -299,8 +302,14 @@ pi_status pi_kv8_read_token(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int
   const pi_kv_layout& L = pool->L;
   PI_REQUIRE(ctx, layer >= 0 && layer < L.num_layers && block >= 0 && block < L.num_blocks && tok >= 0 && tok < L.block_size,
              "KV address (layer %d, block %d, token %d) out of range", layer, block, tok);
-  std::vector<uint8_t> codes((size_t)L.num_kv_heads * 2 * pool->pitch);
-  std::vector<float> scales((size_t)L.num_kv_heads * 2);
+  std::vector<uint8_t> codes;
+  std::vector<float> scales;
+  try {
+    codes.resize((size_t)L.num_kv_heads * 2 * pool->pitch);
+    scales.resize((size_t)L.num_kv_heads * 2);
+  } catch (const std::bad_alloc&) {
+    return pi_fail(ctx, PI_ERR_OOM, "host allocation failed");
+  }
   const size_t tile = ((size_t)layer * L.num_blocks + block) * L.num_kv_heads * 2;
   PI_CUDA(ctx, cudaMemcpy2DAsync(codes.data(), pool->pitch, pool->codes + tile * L.block_size * pool->pitch + (size_t)tok * pool->pitch, (size_t)L.block_size * pool->pitch,
                                  pool->pitch, (size_t)L.num_kv_heads * 2, cudaMemcpyDeviceToHost, ctx->stream));

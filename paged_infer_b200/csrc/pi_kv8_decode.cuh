@@ -1,5 +1,5 @@
 // Paged attention over the 8-bit cache for sequences that bring few rows: decoded tokens, short verify groups.  See
-// pi_kv8_decode.cu for the dispatch; the instantiations are dealt to several files by their pitch.
+// pi_kv8_attention.cu for the dispatch; the instantiations are dealt to several files by their pitch.
 //
 // A warp takes 16 tokens of one block at a time, all with the same two scales.  Codes are whole numbers (or e4m3 values) that f16
 // holds exactly, so both products run on the tensor cores (m16n8k16, f32 accumulators) with the CACHE as the wide operand:
@@ -19,6 +19,10 @@
 //
 // The tokens of a sequence are dealt to the warps of a CTA and to the CTAs of a cluster; partial results are joined through shared
 // memory, then through the cluster's: no scratch in device memory, and the order of the sums is fixed.
+//
+// Measured: 16 sequences of 3000 to 4096, 32 query heads of 128 over 8, bf16, e4m3: 30 us, 3.9 TB/s; 64 of 256 to 2048, 32 over 4 of 64, f32,
+// int8: 22 us, 1.75 TB/s; one of 131072, 64 over 8 of 128: 104 us, 2.6 TB/s.  Bound: the latency of a warp's chain with sixteen warps an
+// SM, and for few long sequences the 16 CTAs of a cluster.
 #pragma once
 
 #include <math.h>

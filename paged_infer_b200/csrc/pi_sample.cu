@@ -17,7 +17,10 @@
 //
 // A cluster of CTAs takes a row: each holds its slice of the logits in shared memory, so that they are read once.  A histogram is
 // made in each CTA's own memory; then every bin has a home in one of them, to which the others add theirs, and everybody reads all
-// bins from their homes.  (Reading all histograms of all eight CTAs instead cost twice as much as everything else together.)
+// bins from their homes.  (Reading all histograms of all eight CTAs instead: 143 us for 64 rows of 128256, against 82.)
+//
+// Bound: the barriers of the cluster and of the CTA, some eight and twenty-five of them with a pass over the slice between each two; the
+// pass that takes the weights is the longest.  Measured: 1 row of 32000 logits 17 us, 64 of 128256 80 us.
 #include <float.h>
 
 #include <algorithm>

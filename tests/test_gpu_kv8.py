@@ -360,6 +360,46 @@ def test_attention_over_strided_rows(ctx):
     assert torch.equal(out2, out) and (wide[:, 557:] == 0).all() and (wide[:, :3] == 0).all()
 
 
+@pytest.mark.parametrize("news", [[1, 1], [40, 1]])
+def test_a_cache_beyond_32_bits(ctx, news):
+    """The same blocks at the front of a small pool and at the end of one of 4.9 GB: the same codes, scales and results."""
+    heads, dim, block, far = 8, 128, 16, 150000
+    rng = np.random.default_rng(2)
+    contexts = np.array([90, 33])
+    after = -(-contexts // block)
+    rows = int(sum(news))
+    q, k, v = (torch.tensor(rng.standard_normal((rows, n, dim)), dtype=torch.bfloat16, device="cuda") for n in (16, heads, heads))
+    small = new_cache(ctx, "int8", 1, 12, heads, block, dim, seed=3)
+    codes = torch.zeros((1, far, heads, 2, block, dim), dtype=torch.int8, device="cuda")
+    scales = torch.ones((1, far, heads, 2), device="cuda")
+    codes[:, far - 12:], scales[:, far - 12:] = small.codes, small.scales
+    large = api.KvCache8(ctx, api.KvLayout(1, far, block, heads, dim), codes=codes, scales=scales)
+    outs = []
+    for cache, shift in ((small, 0), (large, far - 12)):
+        ids = rng.permutation(12)[: after.sum()] if not outs else ids
+        tables = np.full((2, 6), -1)
+        tables[0, : after[0]], tables[1, : after[1]] = ids[: after[0]] + shift, ids[after[0]:] + shift
+        pos = np.concatenate([np.arange(c - n, c) for c, n in zip(contexts, news)])
+        seq = np.repeat([0, 1], news)
+        slots = torch.tensor(tables[seq, pos // block] * block + pos % block, dtype=torch.int64, device="cuda")
+        plan = api.StepPlan(ctx, block, i32(tables), lens=i32(after), cu_rows=i32([0, news[0], rows]), row_pos=i32(pos), slots=slots)
+        cache.write(plan, k, v)
+        out = torch.zeros_like(q)
+        api.PagedAttention8(cache.layout, 16).run_device(q, out, cache, plan)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(large.codes[:, far - 12:], small.codes) and torch.equal(large.scales[:, far - 12:], small.scales)
+    assert (large.codes[:, : far - 12] == 0).all()
+
+
+def test_attention_in_place(ctx):
+    """Results may replace the queries."""
+    for contexts, news in (([300, 40], [1, 1]), ([2000], [40]), ([400], [200])):
+        q, out, cache, plan, given = attention_case(ctx, "int8", "bf16", 16, 8, 2, 64, contexts, news, seed=8)
+        same = q.clone()
+        api.PagedAttention8(cache.layout, 8).run_device(same, same, cache, plan, layer=1, max_seq_rows=int(max(news)), max_context=int(max(contexts)))
+        assert torch.equal(same, out)
+
+
 def test_attention_refusals(ctx):
     q, out, cache, plan, _ = attention_case(ctx, "int8", "f32", 16, 4, 2, 64, [20], [2], seed=1)
     a = api.PagedAttention8(cache.layout, 4)
