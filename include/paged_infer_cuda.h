@@ -575,7 +575,7 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
  * of `arrays` are read (the others may be NULL), of its first n_seqs sequences; rows outside every sequence are not written.
  * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut,
  * and with that the order of sums; results are right whatever they say.  At most 65535 sequences, and as many tiles of
- * 128 (row, head) pairs. */
+ * 16 (row, query head) pairs of one KV head in a sequence.  out may be q itself. */
 pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int num_heads, int dtype, const void* q_dev, size_t q_stride,
                            void* out_dev, size_t out_stride, const pi_step_arrays* arrays, int n_seqs, int n_rows, int max_seq_rows,
                            int max_context, int window, float scale);

@@ -673,7 +673,7 @@ class PagedAttention8:
             _invalid(f"a window of {window} positions")
         check(_lib.lib().pi_kv8_attention(ctx.handle, cache.handle, layer, self.num_heads, kind, q_at, q_row, out_at, out_row, plan._ref, plan.n_seqs, rows,
                                           max(rows, 1) if max_seq_rows is None else max_seq_rows,
-                                          plan._c.max_blocks * plan.block_size if max_context is None else max_context, window or 0,
+                                          plan._c.max_blocks * plan.block_size if max_context is None else max_context, min(window or 0, 2**31 - 1),
                                           L.head_dim ** -0.5 if scale is None else scale), ctx.handle)
 
 

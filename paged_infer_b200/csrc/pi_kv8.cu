@@ -246,6 +246,8 @@ pi_status pi_kv8_pool_create(pi_ctx* ctx, const pi_kv_layout* layout, int kind, 
              layout->num_kv_heads);
   PI_REQUIRE(ctx, !codes_dev_or_null == !scales_dev_or_null, "codes and scales are either both the caller's or both the pool's");
   PI_REQUIRE(ctx, ((uintptr_t)codes_dev_or_null & 15) == 0 && ((uintptr_t)scales_dev_or_null & 7) == 0, "codes must lie on a 16-byte boundary, scales on an 8-byte one");
+  const double bytes_wanted = (double)layout->num_layers * layout->num_blocks * layout->num_kv_heads * 2 * layout->block_size * pi_kv8_pitch_of(layout->head_dim);
+  PI_REQUIRE(ctx, bytes_wanted < 1e15, "a pool of %g bytes", bytes_wanted);   // sizes and offsets fit 64 bits
   pi_kv8_pool* pool = new (std::nothrow) pi_kv8_pool();
   if (!pool) return pi_fail(ctx, PI_ERR_OOM, "host allocation failed");
   pool->L = *layout;

@@ -50,12 +50,13 @@ extern "C" pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int 
   PI_REQUIRE(ctx, a->block_size == L.block_size, "the step's blocks hold %d tokens, the pool's %d", a->block_size, L.block_size);
   PI_REQUIRE(ctx, a->max_blocks > 0 && n_seqs <= a->max_seqs && n_rows <= a->max_rows, "%d sequences and %d rows: the step's arrays have room for %d and %d", n_seqs, n_rows,
              a->max_seqs, a->max_rows);
+  PI_REQUIRE(ctx, (long long)n_rows * num_heads / L.num_kv_heads <= 0x7fffffffll - 4096, "%d rows of %d query heads are too many", n_rows, num_heads);
   PI_REQUIRE(ctx, (long long)a->max_blocks * L.block_size <= 0x7fffffffll - 4096, "tables of %d blocks of %d tokens reach beyond position 2^31", a->max_blocks, L.block_size);
   const size_t row = (size_t)num_heads * L.head_dim, size = dtype == PI_F32 ? 4 : 2;
   PI_REQUIRE(ctx, (q_stride >= row && out_stride >= row) || n_rows == 1, "rows of %zu values cannot be %zu (queries) and %zu (results) apart", row, q_stride, out_stride);
   PI_REQUIRE(ctx, ((uintptr_t)q_dev | (uintptr_t)out_dev) % size == 0, "queries and results must be aligned to their type");
   PI_REQUIRE(ctx, max_seq_rows > 0 && max_context > 0, "the most rows of a sequence and the longest context must be positive");
-  PI_REQUIRE(ctx, scale > 0.f && scale < INFINITY, "a scale of %g", (double)scale);
+  PI_REQUIRE(ctx, scale > 0.f && scale * 1.4426950408889634f < INFINITY, "a scale of %g", (double)scale);
   pi_kv8_attn_params p = {};
   p.q = q_dev;
   p.out = out_dev;

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
   pi_grid_dependency_wait();
   const int row_begin = max(0, min(p.cu_rows[seq], p.n_rows)), row_end = min(p.cu_rows[seq + 1], p.n_rows);
   const int ncols = (row_end - row_begin) * p.group > p.max_cols ? 0 : (row_end - row_begin) * p.group;
-  const int last_token = (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1;
+  const int last_token = max(0, min(p.lens[seq], p.max_blocks)) * bs - 1;
   const int32_t* table = p.tables + (size_t)seq * p.max_blocks;
   // one tile of columns as the grid is cut; the loop is for sequences that bring more rows than the call said
   for (int col0 = blockIdx.z * COLS; col0 < ncols; col0 += gridDim.z * COLS) {
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
     int lo_all = 0x7fffffff, hi_all = -1, lo_most = 0, hi_least = 0x7fffffff;
     const int first_row = row_begin + p.by_group(col0), last_row = row_begin + p.by_group(min(ncols, col0 + COLS) - 1);
     for (int r = first_row; r <= last_row; ++r) {
-      const int pos = p.row_pos[r], from = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+      const int pos = p.row_pos[r], from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
       if (pos >= 0) lo_all = min(lo_all, from);
       hi_all = max(hi_all, pos);
       lo_most = max(lo_most, from);
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
       }
       if (l8 == 0) {
         const int pos = live ? p.row_pos[row] : -1;
-        s_lo[c] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+        s_lo[c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         s_hi[c] = pos;
         s_factor[c] = __uint_as_float((e + 1) << 23) * p.scale2;   // 2^(e - 126)
         s_bias[c] = -kBias * bias;

@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   int pos = -1, from = 0;
   if (live) {
     pos = p.row_pos[s_first + local];
-    from = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+    from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
     if (pos >= 0) {
       atomicMin(&s_lo, from);
       atomicMax(&s_hi, pos);
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   pi_grid_launch_dependents();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem, smem_base = s_u32(smem), lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  const int lo_all = s_lo, hi_all = min(s_hi, (int)min((long long)p.lens[seq], (long long)p.max_blocks) * bs - 1);
+  const int lo_all = s_lo, hi_all = min(s_hi, max(0, min(p.lens[seq], p.max_blocks)) * bs - 1);
   const int per_block = (bs + 15) >> 4, first_block = hi_all < lo_all ? 0 : p.by_block(lo_all);
   const int groups = hi_all < lo_all ? 0 : (p.by_block(hi_all) - first_block + 1) * per_block, tiles_all = (groups + L::groups - 1) / L::groups;
   // this CTA's share of the positions: every splits-th tile
@@ -675,7 +675,7 @@ pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_k
   p.min_cols = min_cols;
   p.err_flag = ctx->dev_err;
   // tiles of rows: each sequence ends with one that may not be full
-  const long long full = (a.n_rows + p.rows_per_tile - 1) / p.rows_per_tile, most = full + std::min(a.n_seqs - 1, a.n_rows - 1);
+  const long long full = ((long long)a.n_rows + p.rows_per_tile - 1) / p.rows_per_tile, most = full + std::min(a.n_seqs - 1, a.n_rows - 1);
   PI_REQUIRE(ctx, most <= 65535, "%lld tiles of rows: at most 65535", most);
   // few tiles share their positions out among clusters, four tiles of them or more to a CTA
   const long long seen = a.window > 0 ? std::min<long long>(max_context, (long long)a.window + a.n_rows) : max_context;

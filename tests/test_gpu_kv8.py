@@ -203,7 +203,8 @@ def test_write_refusals_and_pool_calls(ctx):
     own.write(rows_plan(ctx, 16, [16]), torch.ones(1, 2, 80, device="cuda"), torch.full((1, 2, 80), -2.0, device="cuda"))
     k1, v1 = own.read_token(0, 1, 0)
     assert np.abs(k1 - 1).max() < 1e-6 and np.abs(v1 + 2).max() < 1e-6
-    for layout in (api.KvLayout(1, 3, 16, 2, 257), api.KvLayout(1, 3, 5000, 2, 64), api.KvLayout(0, 3, 16, 2, 64)):
+    huge = 2**31 - 1
+    for layout in (api.KvLayout(1, 3, 16, 2, 257), api.KvLayout(1, 3, 5000, 2, 64), api.KvLayout(0, 3, 16, 2, 64), api.KvLayout(huge, huge, 4096, 1024, 256)):
         with refused():
             api.KvCache8(ctx, layout)
     with refused():
@@ -400,10 +401,28 @@ def test_attention_in_place(ctx):
         assert torch.equal(same, out)
 
 
+def test_attention_of_windows_and_lengths_out_of_any_range(ctx):
+    """A window beyond 32 bits is none; tables of a negative length hold nothing; positions up to 2^31 - 1 see what is mapped of their window."""
+    for news in ([1, 1, 1], [3, 40, 20]):
+        q, out, cache, plan, given = attention_case(ctx, "int8", "bf16", 16, 8, 2, 64, [300, 40, 90], news, seed=9)
+        a, cut = api.PagedAttention8(cache.layout, 8), dict(max_seq_rows=max(news), max_context=300)
+        for window in (2**31 - 1, 2**32 + 1):
+            same = torch.full_like(out, 7.0)
+            a.run_device(q, same, cache, plan, layer=1, window=window, **cut)
+            assert torch.equal(same, out)
+        given.update(lens=np.array([given["lens"][0], 0, 0]), window=2**31 - 200)
+        given["pos"] = np.where(np.arange(sum(news)) < news[0], 2**31 - 1, given["pos"])
+        plan = api.StepPlan(ctx, 16, plan.tables, lens=i32([given["lens"][0], -1, -(2**27) - 1]), cu_rows=plan.cu_rows, row_pos=i32(given["pos"]))
+        again = torch.full_like(out, 7.0)
+        a.run_device(q, again, cache, plan, layer=1, window=given["window"], **cut)
+        given["window"], given["pos"] = 304 - 200, np.where(given["pos"] == 2**31 - 1, 303, given["pos"])   # positions 200 to 303, as before
+        check_attention(q, again, cache, given, q.shape[0], "bf16")
+
+
 def test_attention_refusals(ctx):
     q, out, cache, plan, _ = attention_case(ctx, "int8", "f32", 16, 4, 2, 64, [20], [2], seed=1)
     a = api.PagedAttention8(cache.layout, 4)
-    for kw in (dict(layer=2), dict(window=0), dict(window=-3), dict(scale=0.0), dict(scale=float("nan")), dict(max_seq_rows=0), dict(max_context=0)):
+    for kw in (dict(layer=2), dict(window=0), dict(window=-3), dict(scale=0.0), dict(scale=float("nan")), dict(scale=3e38), dict(max_seq_rows=0), dict(max_context=0)):
         with refused():
             a.run_device(q, out, cache, plan, **kw)
     for x, y, p in ((q.bfloat16(), out, plan), (q[:1], out, plan), (q.cpu(), out, plan), (q[:, :3], out[:, :3], plan), (q, out, api.StepPlan(ctx, 16, plan.tables)),
