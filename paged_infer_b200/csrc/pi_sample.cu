@@ -17,10 +17,10 @@
 //
 // A cluster of CTAs takes a row: each holds its slice of the logits in shared memory, so that they are read once.  A histogram is
 // made in each CTA's own memory; then every bin has a home in one of them, to which the others add theirs, and everybody reads all
-// bins from their homes.  (Reading all histograms of all eight CTAs instead: 143 us for 64 rows of 128256, against 82.)
+// bins from their homes.  (Reading all histograms of all eight CTAs instead: 143 us for 64 rows of 128256 when this took 82.)
 //
 // Bound: the barriers of the cluster and of the CTA, some eight and twenty-five of them with a pass over the slice between each two; the
-// pass that takes the weights is the longest.  Measured: 1 row of 32000 logits 17 us, 64 of 128256 80 us.
+// pass that takes the weights is the longest.  Measured: 1 row of 32000 logits 16 us, 64 of 128256 71 us.
 #include <float.h>
 
 #include <algorithm>
@@ -32,6 +32,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2 * kThreads, kBinBits = 10, kMaxCluster = 8;   // two bins per thread
 constexpr int kWeightBits = 45, kLimb = 15;
 constexpr int kSliceFloats = 48 * 1024;   // logits that fit a CTA's shared memory beside the histograms
+constexpr int kAtOnce = 4;                // weights that a thread takes at a time
 constexpr int kTable = 64;                // floats that 32 doubles take
 
 struct SampleParams {
@@ -92,6 +93,12 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
   return v;
 }
 
+__device__ __forceinline__ unsigned long long cluster_sum(unsigned long long v) {   // of eight neighbouring lanes
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // 2^(j / 32)
 __device__ const double kRoots[32] = {1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
                                       1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
@@ -104,17 +111,12 @@ struct Row {
   const float* x;       // the slice
   int count;
   float most, scale;    // bins per unit of logit
-  double rate, offset;  // log2(e) / T, and minus that times `most`
+  double top, rate;     // `most`, log2(e) / T
   // 2^y for y = (v - most) rate <= 0: a 32nd from the table, the rest g, |g| <= 1/64, by its series up to g^5 (the next term is below 2^-48),
-  // as a multiple of 2^-45
-  __device__ __forceinline__ unsigned long long weight(float v) const {
+  // as a multiple of 2^-45; y above -60
+  __device__ __forceinline__ double exponent(float v) const { return ((double)fminf(v, FLT_MAX) - top) * rate; }   // infinite logits: the largest alone
+  __device__ __forceinline__ double power(double y) const {
     extern __shared__ __align__(16) float s_slice[];
-    if (v == most) return 1ull << kWeightBits;
-    // f32 to f64 by its bits; what is below the normal range counts as 0
-    const uint32_t bits = __float_as_uint(v), mag = bits & 0x7fffffffu;
-    const double wide = mag < 0x00800000u ? 0.0 : __hiloint2double((int)((bits & 0x80000000u) | ((mag >> 3) + (896u << 20))), (int)(bits << 29));
-    const double y = fma(wide, rate, offset);
-    if (!(y > -60.0)) return 0;
     const double shifted = y + 211106232532992.0;                  // 1.5 2^47: the low bits of the sum count 32nds
     const int k = __double2loint(shifted);
     const double g = y - (shifted - 211106232532992.0);
@@ -123,13 +125,37 @@ struct Row {
     e = fma(e, g, 5.5504108664821576e-2);
     e = fma(e, g, 2.402265069591007e-1);
     e = fma(e, g, 6.931471805599453e-1);
-    const double root = reinterpret_cast<const double*>(s_slice)[k & 31];   // the table lies in front of the slice
+    const double root = reinterpret_cast<const double*>(s_slice)[k & 31];   // times 2^45; the table lies in front of the slice
     e = fma(e * g, root, root);
-    const int n = (k >> 5) + kWeightBits;                          // times 2^n, n >= -15
-    const double w = __hiloint2double(__double2hiint(e) + (n << 20), __double2loint(e)) + 4503599627370496.0;   // 2^52: rounds to a whole number
-    return (unsigned long long)__double_as_longlong(w) & 0xfffffffffffffull;
+    const double w = __hiloint2double(__double2hiint(e) + ((k & ~31) << 15), __double2loint(e));   // times 2^floor(y)
+    return (w + 4503599627370496.0) - 4503599627370496.0;          // 2^52: rounds to a whole number
   }
-  __device__ __forceinline__ int bin(float v) const { return min(kBins - 1, (int)((most - v) * scale)); }   // never falls as v does
+  __device__ __forceinline__ unsigned long long weight(float v) const { return exponent(v) > -60.0 ? (unsigned long long)power(exponent(v)) : 0; }
+  // use(logit, weight) for the tokens i, i + 32, ... below `end` with least < logit <= most_used, several at a time, so that the chains of
+  // their weights overlap; they are at least `bound`, with a y above -47.  A thread's sums of weights are exact in f64: at most 96 of them, of
+  // 2^45 at most.  The whole warp calls it.
+  template <typename F>
+  __device__ __forceinline__ void weigh(int i, int end, float least, float most_used, F use) const {
+    const int lane = threadIdx.x & 31;
+    for (; i - lane < end; i += 32 * kAtOnce) {
+      float v[kAtOnce];
+      bool in[kAtOnce], any = false;
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        v[e] = i + 32 * e < end ? x[i + 32 * e] : -INFINITY;
+        any |= in[e] = v[e] > least && !(v[e] > most_used);
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+      double w[kAtOnce];
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) w[e] = power(exponent(v[e]));
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e)
+        if (in[e]) use(v[e], w[e]);
+    }
+  }
+  // Never falls as v does.  The truncated sum's low bits are a whole number; the last bin for what is not a number (infinity minus itself).
+  __device__ __forceinline__ int bin(float v) const { return min(kBins - 1, (int)(__float_as_uint(__fmaf_rz(most - v, scale, 8388608.f)) - 0x4b000000u)); }
 };
 
 struct Shared {
@@ -139,8 +165,9 @@ struct Shared {
   float warp_f[kWarps];
   unsigned int warp_b[kWarps];
   Shown shown;
-  unsigned long long above;
+  unsigned long long above, taken;
   int bin;
+  int2 dealt;
 };
 
 // Running sums over the threads of the CTA; `all`: of all of them.
@@ -257,8 +284,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int from = min((int)rank * p.per, p.n), count = min(p.per, p.n - from);
   const size_t base = (size_t)r * p.stride + from;
   float* const slice = s_slice + kTable + 6 * kBins / ranks;
-  if (tid < 32) reinterpret_cast<double*>(s_slice)[tid] = kRoots[tid];
+  if (tid < 32) reinterpret_cast<double*>(s_slice)[tid] = kRoots[tid] * (double)(1ull << kWeightBits);
   pi_grid_dependency_wait();
+  const float temperature = p.temperature[r], min_p = p.min_p[r], top_p = p.top_p[r], u = p.u[r];
+  const int k = p.top_k[r];
 
   // the slice, and the largest logit; NaN counts as minus infinity, -0 as 0
   float best = -INFINITY;
@@ -294,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
   cluster_sync();
   const uint32_t high = __reduce_max_sync(0xffffffffu, lane < ranks ? peer(&s.shown.most, lane) : 0);
-  const float most = from_ordered(high), temperature = p.temperature[r];
+  const float most = from_ordered(high);
   if (!(temperature > 0.f) || most == -INFINITY) {   // the largest, the lowest index of equal ones; a row without any
     for (int i = tid; i < count; i += kThreads)
       if (slice[i] == most) {
@@ -313,15 +342,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   }
   // tokens below `bound` weigh less than half a unit, or less than min_p
   double exact_bound = (double)most - 32.0 * (double)temperature;
-  const float min_p = p.min_p[r];
   if (min_p > 0.f) exact_bound = max(exact_bound, (double)most + (double)temperature * log(min((double)min_p, 1.0)));
   const float bound = most == INFINITY ? INFINITY : max(__double2float_ru(exact_bound), -FLT_MAX);
   const double rate = 1.4426950408889634 / (double)temperature;
-  // (rates that overflow leave the largest logit alone: everything else weighs 0)
-  const Row row = {slice, count, most, (float)kBins / (most - bound), rate, -(double)most * rate};
+  const Row row = {slice, count, most, most > bound ? (float)kBins / (most - bound) : 0.f, (double)fminf(most, FLT_MAX), rate};
 
-  const int k = p.top_k[r];
-  const float top_p = p.top_p[r];
   const bool by_count = k > 0 && k < p.n, by_weight = top_p < 1.f;
   // kept: above thr, and the first `ties` that equal it; the number below 0 is not -0, which equals it
   uint32_t thr = ordered(bound) - (bound == 0.f ? 2 : 1);
@@ -394,25 +419,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         if (round >= 6) first = 0, last = last_bin;   // whatever the estimate says
         // exact sums: a run of the slice per warp, so that they serve the draw as well
         const int run = ((count + kWarps * 32 - 1) / (kWarps * 32)) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
-        unsigned long long in_front = 0, in = 0, behind = 0;
+        double front_of = 0, in_of = 0, all_of = 0;
         const float least = from_ordered(thr);
-#pragma unroll 2
-        for (int i = i0 + lane; i < i1; i += 32) {
-          const float x = slice[i];
-          if (x > least) {
-            const int b = row.bin(x);
-            const unsigned long long w = row.weight(x);
-            if (b < first) in_front += w;
-            else if (b <= last) in += w;
-            else behind += w;
-          }
-        }
-        in_front = warp_sum(in_front);
-        in = warp_sum(in);
-        behind = warp_sum(behind);
+        row.weigh(i0 + lane, i1, least, INFINITY, [&](float x, double w) {
+          const int b = row.bin(x);
+          all_of += w;
+          if (b < first) front_of += w;
+          if (b >= first && b <= last) in_of += w;
+        });
+        const unsigned long long in_front = warp_sum((unsigned long long)front_of), in = warp_sum((unsigned long long)in_of), in_all = warp_sum((unsigned long long)all_of);
         if (lane == 0) {
           s.warp_sum[warp] = in_front;
-          s.warp_s[0][warp] = in_front + in + behind;
+          s.warp_s[0][warp] = in_all;
           s.warp_s[1][warp] = in_front;
           s.warp_s[2][warp] = in;
         }
@@ -424,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         cluster_sync();
         unsigned long long t[3] = {low_weight, low_bin < first ? low_weight : 0, low_bin >= first && low_bin <= last ? low_weight : 0};
 #pragma unroll
-        for (int e = 0; e < 3; ++e) t[e] += warp_sum(lane < ranks ? peer(&s.shown.sums[round & 1][e], lane) : 0);
+        for (int e = 0; e < 3; ++e) t[e] += cluster_sum((lane & 7) < ranks ? peer(&s.shown.sums[round & 1][e], lane & 7) : 0);
         want = min(max(1ull, (unsigned long long)ceil((double)fmaxf(top_p, 0.f) * (double)t[0])), t[0]);
         interval_above = t[1];
         inside = t[2];
@@ -441,34 +459,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       const uint32_t low = thr;
       thr = refine<true>(row, s, first, last, max(low, last == last_bin ? low : lower(last)), upper(first), low, low_weight, want, turn, above);
       const unsigned long long w = row.weight(from_ordered(thr));
-      ties = (want - above + w - 1) / w;
+      ties = want - above <= w ? 1 : (want - above + w - 1) / w;
     }
   }
 
-  // sums in the order of the indices: a run of the slice per warp
-  const int run = ((count + kWarps * 32 - 1) / (kWarps * 32)) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
-  unsigned long long sum = 0;
-  unsigned int same = 0;
+  // sums in the order of the indices, a run of start .. end per warp, of the tokens of bins from `ahead_of` on, which lie at or below `most_used`
   const float least = from_ordered(thr);
+  int i0, i1;
+  auto sum_run = [&](int start, int end, int ahead_of, float most_used) {
+    const int run = (end - start + kThreads - 1) / kThreads * 32;
+    i0 = min(start + warp * run, end), i1 = min(i0 + run, end);
+    double sum_of = 0;
+    unsigned int same = 0;
+    row.weigh(i0 + lane, i1, least, most_used, [&](float x, double w) {
+      if (row.bin(x) >= ahead_of) sum_of += w;
+    });
+    if (ties > 0)
 #pragma unroll 4
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const float x = slice[i];
-    if (x > least && !(x > sure) && row.bin(x) >= first) sum += row.weight(x);
-    same += x == least;
-  }
-  sum = warp_sum(sum);
-  same = __reduce_add_sync(0xffffffffu, same);
+      for (int i = i0 + lane; i < i1; i += 32) same += slice[i] == least;
+    const unsigned long long sum = warp_sum((unsigned long long)sum_of);
+    same = __reduce_add_sync(0xffffffffu, same);
+    if (lane == 0) {
+      s.warp_a[warp] = sum + (ahead_of > 0 ? s.warp_sum[warp] : 0);
+      s.warp_b[warp] = same;
+    }
+  };
   __syncthreads();
-  if (lane == 0) {
-    s.warp_a[warp] = sum + (first > 0 ? s.warp_sum[warp] : 0);
-    s.warp_b[warp] = same;
-  }
+  sum_run(0, count, first, sure);
   __syncthreads();
-  const unsigned long long in_warp = lane < kWarps ? s.warp_a[lane] : 0;   // lane w looks at warp w
-  const unsigned int equal_in_warp = lane < kWarps ? s.warp_b[lane] : 0;
-  if (warp == 0) {
-    const unsigned long long a = warp_sum(in_warp);
-    const unsigned int b = __reduce_add_sync(0xffffffffu, equal_in_warp);
+  if (warp == 0) {   // lane w looks at warp w
+    const unsigned long long a = warp_sum(lane < kWarps ? s.warp_a[lane] : 0);
+    const unsigned int b = __reduce_add_sync(0xffffffffu, lane < kWarps ? s.warp_b[lane] : 0);
     if (lane == 0) {
       s.shown.weight = a;
       s.shown.ties = b;
@@ -484,50 +505,68 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     if (lane >= o) upto_equals += t;
   }
   const unsigned long long used = min((unsigned long long)(upto_equals - equals), ties), held = (lane < ranks ? peer(&s.shown.weight, lane) : 0) + (min((unsigned long long)upto_equals, ties) - used) * w_thr;
-  const unsigned long long total = warp_sum(lane < ranks ? held : 0), ahead = warp_sum(lane < rank ? held : 0), used_here = __shfl_sync(0xffffffffu, used, rank);
-  const float u = p.u[r];
+  const unsigned long long total = warp_sum(lane < ranks ? held : 0), ahead = warp_sum(lane < rank ? held : 0), used_here = __shfl_sync(0xffffffffu, used, rank), held_here = __shfl_sync(0xffffffffu, held, rank);
   unsigned long long goal = u > 0.f ? (unsigned long long)floor((double)u * (double)total) : 0;
   goal = min(goal, total - 1);
-  // the first token whose running sum exceeds the goal: the warp whose run holds it finds it
-  unsigned int upto_equal = equal_in_warp;
+  // the first token whose running sum exceeds the goal: its CTA finds the warp whose run holds it, deals that run to all warps, and the
+  // warp whose part holds it scans that.  (64 rows of 128256 without top-k or top-p:
+  // 49 us, 60 where that warp scans its whole run.)
+  if (goal >= ahead && goal < ahead + held_here) {
+    unsigned long long before = ahead, taken = used_here;
+    for (bool dealt = false;; dealt = true) {
+      const unsigned long long in_warp = lane < kWarps ? s.warp_a[lane] : 0;
+      const unsigned int equal_in_warp = lane < kWarps ? s.warp_b[lane] : 0;
+      unsigned int upto_equal = equal_in_warp;
 #pragma unroll
-  for (int o = 1; o < kWarps; o <<= 1) {
-    const unsigned int t = __shfl_up_sync(0xffffffffu, upto_equal, o);
-    if (lane >= o) upto_equal += t;
-  }
-  const unsigned long long taken_upto = min(used_here + upto_equal, ties), taken_before = min(used_here + (upto_equal - equal_in_warp), ties);
-  const unsigned long long holds = in_warp + (taken_upto - taken_before) * w_thr;
-  unsigned long long holds_upto = holds;
-#pragma unroll
-  for (int o = 1; o < kWarps; o <<= 1) {
-    const unsigned long long t = __shfl_up_sync(0xffffffffu, holds_upto, o);
-    if (lane >= o) holds_upto += t;
-  }
-  unsigned long long mine = ahead + __shfl_sync(0xffffffffu, holds_upto - holds, warp), taken = __shfl_sync(0xffffffffu, taken_before, warp);
-  const unsigned long long here = __shfl_sync(0xffffffffu, holds, warp);
-  if (goal >= mine && goal < mine + here) {
-    for (int i = i0 + lane; i - lane < i1; i += 32) {
-      const float x = i < i1 ? slice[i] : -INFINITY;
-      const unsigned equal = __ballot_sync(0xffffffffu, i < i1 && x == least);
-      unsigned long long w = 0;
-      if (x > least) w = row.weight(x);
-      if (i < i1 && x == least && taken + __popc(equal & ((1u << lane) - 1)) < ties) w = w_thr;
-      taken += __popc(equal);
-      unsigned long long upto = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long t = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += t;
+      for (int o = 1; o < kWarps; o <<= 1) {
+        const unsigned int t = __shfl_up_sync(0xffffffffu, upto_equal, o);
+        if (lane >= o) upto_equal += t;
       }
-      const unsigned found = __ballot_sync(0xffffffffu, mine + upto > goal);
-      if (found) {
-        if (lane == __ffs(found) - 1) {
-          p.ids[r] = from + i;
-          if (p.probs) p.probs[r] = (float)((double)w / (double)total);
+      const unsigned long long taken_before = min(taken + (upto_equal - equal_in_warp), ties), holds = in_warp + (min(taken + upto_equal, ties) - taken_before) * w_thr;
+      unsigned long long holds_upto = holds;
+#pragma unroll
+      for (int o = 1; o < kWarps; o <<= 1) {
+        const unsigned long long t = __shfl_up_sync(0xffffffffu, holds_upto, o);
+        if (lane >= o) holds_upto += t;
+      }
+      unsigned long long mine = before + __shfl_sync(0xffffffffu, holds_upto - holds, warp), taken_mine = __shfl_sync(0xffffffffu, taken_before, warp);
+      const bool here = goal >= mine && goal < mine + __shfl_sync(0xffffffffu, holds, warp);
+      if (dealt) {
+        for (int i = i0 + lane; here && i - lane < i1; i += 32) {
+          const float x = i < i1 ? slice[i] : -INFINITY;
+          const unsigned equal = __ballot_sync(0xffffffffu, i < i1 && x == least);
+          unsigned long long w = 0;
+          if (x > least) w = row.weight(x);
+          if (i < i1 && x == least && taken_mine + __popc(equal & ((1u << lane) - 1)) < ties) w = w_thr;
+          taken_mine += __popc(equal);
+          unsigned long long upto = w;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+          }
+          const unsigned found = __ballot_sync(0xffffffffu, mine + upto > goal);
+          if (found) {
+            if (lane == __ffs(found) - 1) {
+              p.ids[r] = from + i;
+              if (p.probs) p.probs[r] = (float)((double)w / (double)total);
+            }
+            break;
+          }
+          mine += __shfl_sync(0xffffffffu, upto, 31);
         }
         break;
       }
-      mine += __shfl_sync(0xffffffffu, upto, 31);
+      if (here && lane == 0) {
+        s.dealt = make_int2(i0, i1);
+        s.above = mine;
+        s.taken = taken_mine;
+      }
+      __syncthreads();
+      before = s.above, taken = s.taken;
+      const int2 dealt_run = s.dealt;
+      sum_run(dealt_run.x, dealt_run.y, 0, INFINITY);
+      __syncthreads();
     }
   }
   cluster_sync();   // nobody leaves while another one reads its memory
