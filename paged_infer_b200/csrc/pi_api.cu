@@ -5,13 +5,63 @@
 #include <string.h>
 
 #include <algorithm>
+#include <mutex>
 #include <new>
 
 #include "pi_layered.cuh"
 
 namespace {
 thread_local std::string g_create_error;
+
+// What contexts of one device share: its properties, asked for once, and their error records, cut from one allocation, so that a
+// context on a stream of the caller's is created without a call to the device and destroyed without cudaFree, which waits for all of
+// the device's streams.  (On a stream of the caller's: 2 us to create and 7 to destroy; with cudaGetDeviceProperties and an allocation each 890, and whatever the device was busy with.)
+constexpr int kDevices = 64, kErrRecords = 256;
+struct DeviceShare {
+  bool known = false;
+  int major = 0, minor = 0, sm_count = 0, smem_optin = 0;
+  int* records = nullptr;             // kErrRecords of PI_DEV_ERR_WORDS, all zero but those in use
+  unsigned char next[kErrRecords];    // records that are free
+  int free = 0;
+};
+std::mutex g_share_mutex;
+DeviceShare g_share[kDevices];
+
+cudaError_t device_facts(int device, DeviceShare& d) {
+  if (d.known) return cudaSuccess;
+  cudaError_t e = cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.minor, cudaDevAttrComputeCapabilityMinor, device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+  d.known = e == cudaSuccess;
+  return e;
 }
+
+// A record of zeros on the current device; its own allocation where the shared ones are all in use.
+cudaError_t take_record(DeviceShare& d, int** out, bool* owned) {
+  const size_t bytes = PI_DEV_ERR_WORDS * sizeof(int);
+  const auto zeros = [](int** at, size_t n) {   // complete on return: the context's stream need not be ordered behind the default one
+    cudaError_t e = cudaMalloc(at, n);
+    if (e != cudaSuccess) return e;
+    e = cudaMemset(*at, 0, n);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+    if (e != cudaSuccess) {
+      cudaFree(*at);
+      *at = nullptr;
+    }
+    return e;
+  };
+  if (!d.records) {
+    const cudaError_t e = zeros(&d.records, kErrRecords * bytes);
+    if (e != cudaSuccess) return e;
+    for (d.free = 0; d.free < kErrRecords; ++d.free) d.next[d.free] = (unsigned char)(kErrRecords - 1 - d.free);
+  }
+  *owned = d.free == 0;
+  if (*owned) return zeros(out, bytes);
+  *out = d.records + (size_t)d.next[--d.free] * PI_DEV_ERR_WORDS;
+  return cudaSuccess;
+}
+}  // namespace
 
 void pi_set_global_error(const char* msg) { g_create_error = msg ? msg : ""; }
 
@@ -118,17 +168,19 @@ static pi_status ctx_create_common(int device, void* stream, pi_ctx** out) {
   if (device < 0 || device >= count) return pi_fail(nullptr, PI_ERR_INVALID_ARG, "device %d of %d", device, count);
   e = cudaSetDevice(device);
   if (e != cudaSuccess) return pi_fail(nullptr, PI_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(e));
-  cudaDeviceProp prop;
-  e = cudaGetDeviceProperties(&prop, device);
-  if (e != cudaSuccess) return pi_fail(nullptr, PI_ERR_CUDA, "cudaGetDeviceProperties: %s", cudaGetErrorString(e));
-  if (prop.major != 10)
+  PI_REQUIRE(nullptr, device < kDevices, "device %d: at most %d are served", device, kDevices);
+  std::lock_guard<std::mutex> lock(g_share_mutex);
+  DeviceShare& share = g_share[device];
+  e = device_facts(device, share);
+  if (e != cudaSuccess) return pi_fail(nullptr, PI_ERR_CUDA, "cudaDeviceGetAttribute: %s", cudaGetErrorString(e));
+  if (share.major != 10)
     return pi_fail(nullptr, PI_ERR_UNSUPPORTED, "device %d is sm_%d%d; this library is built for sm_100a only", device,
-                   prop.major, prop.minor);
+                   share.major, share.minor);
   pi_ctx* ctx = new (std::nothrow) pi_ctx();
   if (!ctx) return pi_fail(nullptr, PI_ERR_OOM, "host allocation failed");
   ctx->device = device;
-  ctx->sm_count = prop.multiProcessorCount;
-  ctx->smem_optin = prop.sharedMemPerBlockOptin;
+  ctx->sm_count = share.sm_count;
+  ctx->smem_optin = (size_t)share.smem_optin;
   if (stream) {
     ctx->stream = static_cast<cudaStream_t>(stream);
   } else {
@@ -139,9 +191,9 @@ static pi_status ctx_create_common(int device, void* stream, pi_ctx** out) {
     }
     ctx->own_stream = true;
   }
-  e = cudaMalloc(&ctx->dev_err, PI_DEV_ERR_WORDS * sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(ctx->dev_err, 0, PI_DEV_ERR_WORDS * sizeof(int));
+  e = take_record(share, &ctx->dev_err, &ctx->own_dev_err);
   if (e != cudaSuccess) {
+    if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return pi_fail(nullptr, PI_ERR_CUDA, "context allocation: %s", cudaGetErrorString(e));
   }
@@ -172,14 +224,22 @@ pi_status pi_ctx_create_tp(int device, void* stream, int rank, int tp, const voi
 void pi_ctx_destroy(pi_ctx* ctx) {
   if (!ctx) return;
   cudaSetDevice(ctx->device);
-  cudaStreamSynchronize(ctx->stream);
+  // behind the context's last kernel its error record is zero again, for the next context
+  bool clean = cudaMemsetAsync(ctx->dev_err, 0, PI_DEV_ERR_WORDS * sizeof(int), ctx->stream) == cudaSuccess;
+  clean = cudaStreamSynchronize(ctx->stream) == cudaSuccess && clean;
   pi_tp_destroy(ctx);
   for (pi_buffer* b : {&ctx->staging_in, &ctx->staging_out, &ctx->attn_tables, &ctx->attn_partial, &ctx->attn_plan, &ctx->gemm_act, &ctx->wide_planes,
                        &ctx->gemm_parked})
     if (b->ptr) cudaFree(b->ptr);
   if (ctx->pinned) cudaFreeHost(ctx->pinned);
   for (cudaEvent_t e : ctx->prof_events) cudaEventDestroy(e);
-  if (ctx->dev_err) cudaFree(ctx->dev_err);
+  if (ctx->own_dev_err) {
+    cudaFree(ctx->dev_err);
+  } else if (clean) {
+    std::lock_guard<std::mutex> lock(g_share_mutex);
+    DeviceShare& share = g_share[ctx->device];
+    share.next[share.free++] = (unsigned char)((ctx->dev_err - share.records) / PI_DEV_ERR_WORDS);
+  }
   if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
   delete ctx;
 }

@@ -73,6 +73,7 @@ struct pi_ctx {
   std::string err;
   uint64_t launches = 0;
   int* dev_err = nullptr;   // device words: [0] set by a kernel that gave up (bounded wait ran out, inconsistent input), [1..] its record
+  bool own_dev_err = false; // an allocation of its own, not one of the device's shared records
 
   // tensor parallelism
   int rank = 0, tp = 1;
