@@ -173,17 +173,17 @@ def prepare(case, seed):
     s = _inputs(case, seed)
     if not own:
         return s
-    # what a program keeps beside its tensors: a context on torch's stream (handle 1 is the legacy default stream), the step's arrays, the cache's handle
+    # what a program keeps beside its tensors: its context, the step's arrays, the cache's handle
     from paged_infer_b200 import api
-    s["api"], s["ctx"] = api, api.Context(torch.cuda.current_device(), stream=torch.cuda.current_stream().cuda_stream or 1)
+    s["api"], s["ctx"] = api, _context(api)
     if case["op"] == "sample":
         return s
     arrays = dict(tables=s["tables"], lens=s.get("lens"), cu_rows=s.get("cu"), row_seq=s.get("seq"), row_pos=s.get("pos"), slots=s.get("slots"))
     new = lambda n, t=torch.int32: torch.empty(n, dtype=t, device="cuda")  # noqa: E731
     if case["op"] == "plan":
         B, cap = case["seqs"], s["cap"]
-        arrays |= dict(lens=new(B), cu_rows=new(B + 1), row_seq=new(cap), row_pos=new(cap), slots=new(cap, torch.int64))
-    s["plan"] = api.StepPlan(s["ctx"], block_size=case["block"], counts=new(3), **arrays)
+        arrays |= dict(lens=new(B), cu_rows=new(B + 1), row_seq=new(cap), row_pos=new(cap), slots=new(cap, torch.int64), counts=new(3))
+    s["plan"] = api.StepPlan(s["ctx"], block_size=case["block"], **arrays)
     if case["op"] != "plan":
         layout = api.KvLayout(LAYERS, s["codes"].shape[1], case["block"], case["kv_heads"], case["dim"])
         s["cache"] = api.KvCache8(s["ctx"], layout, codes=s["codes"], scales=s["scales"])
@@ -191,6 +191,17 @@ def prepare(case, seed):
         s["attention"] = api.PagedAttention8(layout, case["heads"])
         s["out"] = torch.empty_like(s["q"])
     return s
+
+
+_contexts = {}                             # a server has one for each of its streams, whatever steps it runs there
+
+
+def _context(api):
+    """The context of torch's current stream (handle 1 is the legacy default stream)."""
+    key = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream or 1
+    if key not in _contexts:
+        _contexts[key] = api.Context(key[0], stream=key[1])
+    return _contexts[key]
 
 
 def _logits(case, seed, g):
