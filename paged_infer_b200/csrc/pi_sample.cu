@@ -110,7 +110,7 @@ __device__ const double kRoots[32] = {1.0, 1.0218971486541166, 1.044273782427413
 struct Row {
   const float* x;       // the slice
   int count;
-  float most, scale;    // bins per unit of logit
+  float most, scale;    // bins per unit of logit; 0: all tokens are in one bin
   double top, rate;     // `most`, log2(e) / T
   // 2^y for y = (v - most) rate <= 0: a 32nd from the table, the rest g, |g| <= 1/64, by its series up to g^5 (the next term is below 2^-48),
   // as a multiple of 2^-45; y above -60
@@ -228,6 +228,10 @@ __device__ uint32_t refine(const Row& row, Shared& s, int first, int last, uint3
     const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
 #pragma unroll
     for (int i = 0; i < (WEIGHT ? 3 : 1); ++i) s.hist[i][tid] = s.hist[i][tid + kThreads] = 0;
+    if (tid == 0) {   // amounts that do not reach `want` leave the smallest
+      s.bin = 0;
+      s.above = above;
+    }
     __syncthreads();
     const float from = from_ordered(lo), to = from_ordered(hi);
 #pragma unroll 4
@@ -343,9 +347,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   // tokens below `bound` weigh less than half a unit, or less than min_p
   double exact_bound = (double)most - 32.0 * (double)temperature;
   if (min_p > 0.f) exact_bound = max(exact_bound, (double)most + (double)temperature * log(min((double)min_p, 1.0)));
-  const float bound = most == INFINITY ? INFINITY : max(__double2float_ru(exact_bound), -FLT_MAX);
+  const float bound = most == INFINITY ? INFINITY : max(__double2float_ru(exact_bound), -FLT_MAX) + 0.f;   // not -0
   const double rate = 1.4426950408889634 / (double)temperature;
-  const Row row = {slice, count, most, most > bound ? (float)kBins / (most - bound) : 0.f, (double)fminf(most, FLT_MAX), rate};
+  // An interval beyond a float's range is cut at that: what lies further down is in the last bin.  One so short (below 3e-36, with
+  // temperatures below 1e-37) that a unit would hold more bins than a float can say is one bin.
+  const float width = fminf(most - bound, FLT_MAX), bins = most > bound ? (float)kBins / width : 0.f;
+  const Row row = {slice, count, most, bins <= FLT_MAX ? bins : 0.f, (double)fminf(most, FLT_MAX), rate};
 
   const bool by_count = k > 0 && k < p.n, by_weight = top_p < 1.f;
   // kept: above thr, and the first `ties` that equal it; the number below 0 is not -0, which equals it
@@ -368,14 +375,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     upto[1] = scan(here[0] + here[1], s.warp_b, all);
     upto[0] = upto[1] - here[1];
     // logits at the edges of a bin, a little outside
-    const float step = (most - bound) / (float)kBins, slack = fmaxf(fabsf(most), fabsf(bound)) * 1e-6f;
+    const float step = width / (float)kBins, slack = fmaxf(fabsf(most), fabsf(bound)) * 1e-6f;
     auto upper = [&](int b) {
       const float x = most - (float)b * step + slack + 0.f;
-      return b == 0 || !(x < most) ? high : ordered(x);
+      return b == 0 || row.scale == 0.f || !(x < most) ? high : ordered(x);
     };
     auto lower = [&](int b) {
       const float x = most - (float)(b + 1) * step - slack + 0.f;
-      return b == kBins - 1 || !(x > bound) ? ordered(bound) : ordered(x);
+      return b == kBins - 1 || row.scale == 0.f || !(x > bound) ? ordered(bound) : ordered(x);
     };
     int last_bin = kBins - 1;
     if (by_count && all > (unsigned int)k) {
@@ -398,8 +405,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       // where the nucleus should end
       float sum;
       float hint[2], hints[2];
+      const float fall = (float)((double)step * row.rate);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) hint[e] = (float)here[e] * exp2f(-((float)(2 * tid + e) + 0.5f) * step * (float)row.rate);
+      for (int e = 0; e < 2; ++e) hint[e] = (float)here[e] * exp2f(-((float)(2 * tid + e) + 0.5f) * fall);
       hints[1] = scan(hint[0] + hint[1], s.warp_f, sum);
       hints[0] = hints[1] - hint[1];
       const unsigned long long low_weight = ties * row.weight(from_ordered(thr));
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         want = min(max(1ull, (unsigned long long)ceil((double)fmaxf(top_p, 0.f) * (double)t[0])), t[0]);
         interval_above = t[1];
         inside = t[2];
-        if (interval_above < want && want <= interval_above + inside) break;
+        if ((interval_above < want && want <= interval_above + inside) || round == 7) break;   // from round 6 on it is all of them
         // the estimate again, from the exact sum in front of the interval
         if (tid == first / 2) s.warp_f[0] = hints[first & 1] - hint[first & 1];
         __syncthreads();
@@ -459,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       const uint32_t low = thr;
       thr = refine<true>(row, s, first, last, max(low, last == last_bin ? low : lower(last)), upper(first), low, low_weight, want, turn, above);
       const unsigned long long w = row.weight(from_ordered(thr));
-      ties = want - above <= w ? 1 : (want - above + w - 1) / w;
+      ties = want - above <= w || w == 0 ? 1 : (want - above + w - 1) / w;
     }
   }
 
