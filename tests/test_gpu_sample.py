@@ -1,4 +1,4 @@
-"""Sampling where the tokens that can be drawn span less or more than a float's range divides."""
+"""Sampling where the tokens that can be drawn span less or more than a float's range divides, and under flat weights."""
 import numpy as np
 import pytest
 import torch
@@ -43,3 +43,15 @@ def test_sample_of_logits_across_the_whole_range(ctx, t):
     x[2] = np.round(x[2] / 4e37) * np.float32(4e37)      # many equal ones
     for k, p, m in KINDS + [(2600, 1, 0), (3500, 0.999, 0)]:
         check_sample(ctx, torch.tensor(x, device="cuda"), t, k, p, m, rng.random(3).astype(np.float32))
+
+
+@pytest.mark.parametrize("t", [1e6, np.inf])
+def test_top_k_of_flat_weights(ctx, t):
+    """Counting does not look at weights."""
+    rng = np.random.default_rng(3)
+    x = torch.tensor(rng.standard_normal((8, 5000)), dtype=torch.float32, device="cuda")
+    x[1] = x[1].round()
+    x[2, 100:] = -float("inf")
+    x[3] = 0.25
+    for k in (1, 2, 7, 40, 1000, 4999):
+        check_sample(ctx, x, t, k, 1, 0, rng.random(8).astype(np.float32))
