@@ -61,25 +61,28 @@ __device__ __forceinline__ void st_shared(uint32_t addr, uint32_t a, uint32_t b,
 }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// A try may suspend the thread for a while that the hardware limits; tries end after kSpinP of them or about a second.
-// Converters, who are ahead, sleep between theirs.
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// A try may suspend the thread for a while that the hardware limits; tries end after kSpinP of them or about a second, or when the CTA
+// gives up.  Converters, who are ahead, sleep between theirs.
 template <bool NAP = false>
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (bar_try(bar, parity)) return true;
   const long long until = clock64() + (1ll << 31);
-  for (uint32_t spin = 0; spin < kSpinP; ++spin) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return true;
+  for (uint32_t spin = 0; spin < kSpinP && !*abort_flag && clock64() < until; ++spin) {
     if (NAP) __nanosleep(200);
-    if (clock64() > until) return false;
+    if (bar_try(bar, parity)) return true;
   }
   return false;
 }
+// Every lane waits for itself: what was released to the barrier is then there for all of them (a shuffle of one lane's answer would
+// order no memory).
 template <bool NAP = false>
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int lane) {
-  int ok = 1;
-  if (lane == 0) ok = (!*abort_flag && bar_wait<NAP>(bar, parity)) ? 1 : 0;
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, bar_wait<NAP>(bar, parity, abort_flag));
 }
 // K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     bool alive = true;
     const int to = min(pos, hi_all);
     auto fold = [&](int j) -> bool {   // the product of tile j into the output
-      if (!warp_wait(o_full, j & 1, &s_abort, lane)) {
+      if (!warp_wait(o_full, j & 1, &s_abort)) {
         if (lane == 0) fail(22);
         return false;
       }
@@ -320,8 +323,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         meet();
         continue;
       }
-      // the scores; what the converters wrote of the groups was released to the thread that issued them
-      if (!warp_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort, lane)) {
+      // the groups, which the converters wrote (the products' thread has waited for them, but its commit hands on only what the products
+      // did; the stage is not filled again before these warps have delivered the tile's weights), and the scores
+      if (!__all_sync(0xffffffffu, bar_wait(kv_full0 + 8 * (j % STAGES), (j / STAGES) & 1, &s_abort) && bar_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort))) {
         if (lane == 0) fail(21);
         alive = false;
         meet();
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const int stg = j % STAGES;
       const Place k_next = locate(j + EVERY, k_token >> 4);
       v_here = locate(j + EVERY, v_eight >> 1);
-      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort, lane)) {
+      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort)) {
         if (lane == 0) fail(23);
         break;
       }
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     auto idesc = [](uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((uint32_t)(kRowsP >> 4) << 24); };   // f16 x f16 -> f32
     auto scores = [&](int j) -> bool {
       const int stg = j % STAGES, buf = j & 1;
-      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / STAGES) & 1)) {
+      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / STAGES) & 1, &s_abort)) {
         fail(24);
         return false;
       }
@@ -606,7 +610,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const int stg = j % STAGES;
       // the next tile's scores run while the row threads work on this tile's
       if (j + 1 < ntiles && !scores(j + 1)) break;
-      if (s_abort || !bar_wait(p_full, j & 1) || (j > 0 && !bar_wait(o_free, (j - 1) & 1))) {
+      if (s_abort || !bar_wait(p_full, j & 1, &s_abort) || (j > 0 && !bar_wait(o_free, (j - 1) & 1, &s_abort))) {
         fail(25);
         break;
       }
