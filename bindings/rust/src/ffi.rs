@@ -26,6 +26,7 @@ pub const PI_OPT_ATTN_SHARED: i32 = 7;
 pub const PI_OPT_PEER_SPIN_LIMIT: i32 = 8;
 pub const PI_OPT_TP_PUSH: i32 = 9;
 pub const PI_OPT_ATTN_FLAT: i32 = 10;
+pub const PI_OPT_KV8_WAIT_LIMIT: i32 = 11;
 pub const PI_SPLIT_NONE: i32 = 0;
 pub const PI_SPLIT_COLUMN: i32 = 1;
 pub const PI_SPLIT_ROW: i32 = 2;

@@ -124,7 +124,8 @@ enum { PI_OPT_TENSOR_GEMM = 1, PI_OPT_CUDA_GRAPH = 2, PI_OPT_PDL = 3, PI_OPT_GEM
        PI_OPT_PEER_SPIN_LIMIT = 8 /* polls, 64 ns apart, that a rank waits for a peer's partial sums; 0 = default */,
        PI_OPT_TP_PUSH = 9 /* peer path: row-split projections store their partial sums into every rank's buffer themselves */,
        PI_OPT_ATTN_FLAT = 10 /* batched decode attention over one flat tile list cut into equal ranges per resident warp:
-                                0 never, 1 (default) inside a model forward, 2 also for a single pi_paged_attention call */ };
+                                0 never, 1 (default) inside a model forward, 2 also for a single pi_paged_attention call */,
+       PI_OPT_KV8_WAIT_LIMIT = 11 /* clocks that a wait between the warps of pi_kv8_attention may take; 0 = default, about a second */ };
 pi_status pi_ctx_set_option(pi_ctx* ctx, int option, int value);
 
 /* ---- quantiser --------------------------------------------------------------- */
@@ -575,7 +576,9 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
  * of `arrays` are read (the others may be NULL), of its first n_seqs sequences; rows outside every sequence are not written.
  * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut,
  * and with that the order of sums; results are right whatever they say.  At most 65535 sequences, and as many tiles of
- * 16 (row, query head) pairs of one KV head in a sequence.  out may be q itself. */
+ * 16 (row, query head) pairs of one KV head in a sequence.  out may be q itself.  Waits inside the kernels are bounded
+ * (PI_OPT_KV8_WAIT_LIMIT): where one runs out the rows concerned become NaN and the next pi_ctx_synchronize returns
+ * PI_ERR_TIMEOUT; a caller that never synchronises through the context sees the NaN alone. */
 pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int num_heads, int dtype, const void* q_dev, size_t q_stride,
                            void* out_dev, size_t out_stride, const pi_step_arrays* arrays, int n_seqs, int n_rows, int max_seq_rows,
                            int max_context, int window, float scale);

@@ -27,6 +27,7 @@ PI_OPT_TENSOR_GEMM, PI_OPT_CUDA_GRAPH, PI_OPT_PDL, PI_OPT_GEMV_MAX_M, PI_OPT_ATT
 PI_OPT_PEER_SPIN_LIMIT = 8
 PI_OPT_TP_PUSH = 9
 PI_OPT_ATTN_FLAT = 10
+PI_OPT_KV8_WAIT_LIMIT = 11
 
 
 class PiError(RuntimeError):

@@ -301,6 +301,10 @@ pi_status pi_ctx_set_option(pi_ctx* ctx, int option, int value) {
       PI_REQUIRE(ctx, value >= 0, "the spin limit cannot be negative");
       ctx->peer_spin_limit = (uint32_t)value;
       return PI_OK;
+    case PI_OPT_KV8_WAIT_LIMIT:
+      PI_REQUIRE(ctx, value >= 0, "the wait limit cannot be negative");
+      ctx->kv8_wait_limit = value;
+      return PI_OK;
     case PI_OPT_GEMV_MAX_M:
       PI_REQUIRE(ctx, value >= 1, "gemv max M must be at least 1");
       ctx->opt_gemv_max_m = value;

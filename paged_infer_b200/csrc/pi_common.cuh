@@ -91,6 +91,7 @@ struct pi_ctx {
     bool pushed = false;                        // the partial sums of the next exchange were pushed into every rank's buffer
   } peer;
   uint32_t peer_spin_limit = 0;   // polls a rank waits for a peer's partial sums; 0 = the default (about a second)
+  int kv8_wait_limit = 0;         // clocks that a wait inside an attention kernel over the 8-bit cache may take; 0 = the default (about a second)
 
   // options
   bool opt_tensor_gemm = true;

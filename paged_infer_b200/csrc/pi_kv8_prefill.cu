@@ -17,7 +17,8 @@
 // tiles), into registers ahead of their turn, then widened into shared memory (V by byte permutes of eight tokens at a time).
 // Warp 16: issues the products (17-19 are there because registers are dealt to four warps at a time); the scores of tile j + 1 run
 // while the rows work on tile j.
-// Hand-offs go through mbarriers; every wait is bounded and raises the context's error word instead of hanging.  Where there are few
+// Hand-offs go through mbarriers; every wait is bounded and raises the context's error word instead of hanging, and the tile's rows
+// become NaN.  Where there are few
 // tiles of rows, a cluster shares the positions of one and joins its CTAs' outputs through shared memory.
 //
 // Bound: the rows' threads.  A tile of 128 by 128 needs 16384 exponentials, of which an SM makes 16 a clock: 1024 clocks, as long as
@@ -38,12 +39,13 @@ namespace {
 using namespace pi_kv8;
 
 constexpr int kRowsP = 128, kPartP = 64, kThreadsP = 20 * 32, kMostStages = 4;   // a part: the tokens of a tile that four warps widen
-constexpr uint32_t kSpinP = 1u << 21;   // polls of a wait
+constexpr long long kWaitLimitP = 1ll << 31;   // clocks of a wait: about a second
 
 struct PrefillParams {
   pi_kv8_attn_params a;
   int rows_per_tile, min_cols;   // rows of a tile; sequences with fewer columns are another kernel's
   int* err_flag;
+  long long wait_limit;          // clocks
 };
 
 // 16 tokens of a tile: first position, how many are there (0: not mapped), scale of K, scale of V as 2^v_exp 2^v_log, v_log in [0, 1).
@@ -66,13 +68,18 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
-// A try may suspend the thread for a while that the hardware limits; tries end after kSpinP of them or about a second, or when the CTA
-// gives up.  Converters, who are ahead, sleep between theirs.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {   // the same without suspending
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// A try may suspend the thread for a while that the hardware limits; tries end after `limit` clocks, or when the CTA gives up.
+// Converters, who are ahead, sleep between theirs.
 template <bool NAP = false>
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (bar_try(bar, parity)) return true;
-  const long long until = clock64() + (1ll << 31);
-  for (uint32_t spin = 0; spin < kSpinP && !*abort_flag && clock64() < until; ++spin) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
+  if (bar_test(bar, parity)) return true;
+  const long long until = clock64() + limit;
+  while (clock64() < until && !(abort_flag && *abort_flag)) {
     if (NAP) __nanosleep(200);
     if (bar_try(bar, parity)) return true;
   }
@@ -81,8 +88,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 // Every lane waits for itself: what was released to the barrier is then there for all of them (a shuffle of one lane's answer would
 // order no memory).
 template <bool NAP = false>
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, bar_wait<NAP>(bar, parity, abort_flag));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
+  return __all_sync(0xffffffffu, bar_wait<NAP>(bar, parity, abort_flag, limit));
 }
 // K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   const pi_kv8_attn_params& p = pp.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) unsigned long long bars[2 * kMostStages + 5];
+  __shared__ __align__(8) unsigned long long bars[2 * kMostStages + 6];
   __shared__ Group s_group[kMostStages][8];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
@@ -145,7 +152,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const int kvh = blockIdx.x / splits;
   const uint32_t kv_full0 = s_u32(&bars[0]), kv_free0 = s_u32(&bars[kMostStages]), s_full0 = s_u32(&bars[2 * kMostStages]), p_full = s_u32(&bars[2 * kMostStages + 2]),
-                 o_full = s_u32(&bars[2 * kMostStages + 3]), o_free = s_u32(&bars[2 * kMostStages + 4]);
+                 o_full = s_u32(&bars[2 * kMostStages + 3]), o_free = s_u32(&bars[2 * kMostStages + 4]), idle = s_u32(&bars[2 * kMostStages + 5]);
   pi_grid_dependency_wait_only();
 
   // the tile of rows: sequences' tiles are numbered through
@@ -189,6 +196,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       bar_init(p_full, 8);               // one arrival per row warp
       bar_init(o_full, 1);
       bar_init(o_free, 8);
+      bar_init(idle, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -292,7 +300,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     bool alive = true;
     const int to = min(pos, hi_all);
     auto fold = [&](int j) -> bool {   // the product of tile j into the output
-      if (!warp_wait(o_full, j & 1, &s_abort)) {
+      if (!warp_wait(o_full, j & 1, &s_abort, pp.wait_limit)) {
         if (lane == 0) fail(22);
         return false;
       }
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       }
       // the groups, which the converters wrote (the products' thread has waited for them, but its commit hands on only what the products
       // did; the stage is not filled again before these warps have delivered the tile's weights), and the scores
-      if (!__all_sync(0xffffffffu, bar_wait(kv_full0 + 8 * (j % STAGES), (j / STAGES) & 1, &s_abort) && bar_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort))) {
+      if (!__all_sync(0xffffffffu, bar_wait(kv_full0 + 8 * (j % STAGES), (j / STAGES) & 1, &s_abort, pp.wait_limit) && bar_wait(s_full0 + 8 * buf, (j >> 1) & 1, &s_abort, pp.wait_limit))) {
         if (lane == 0) fail(21);
         alive = false;
         meet();
@@ -439,7 +447,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       __syncwarp();
       if (lane == 0) bar_arrive(p_full);
     }
-    if (alive && ntiles > 0) fold(ntiles - 1);
+    if (alive && ntiles > 0) alive = fold(ntiles - 1);
+    if (!alive) sum = NAN;   // a wait ran out: the row's results say so, whatever CTA they come from
     // the halves' sums, in the buffer that the last tile did not use
     s_most[ntiles & 1][half][m] = sum;
     meet();
@@ -529,7 +538,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const int stg = j % STAGES;
       const Place k_next = locate(j + EVERY, k_token >> 4);
       v_here = locate(j + EVERY, v_eight >> 1);
-      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort)) {
+      if (!warp_wait<true>(kv_free0 + 8 * stg, ((j / STAGES) & 1) ^ 1, &s_abort, pp.wait_limit)) {
         if (lane == 0) fail(23);
         break;
       }
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     auto idesc = [](uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((uint32_t)(kRowsP >> 4) << 24); };   // f16 x f16 -> f32
     auto scores = [&](int j) -> bool {
       const int stg = j % STAGES, buf = j & 1;
-      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / STAGES) & 1, &s_abort)) {
+      if (s_abort || !bar_wait(kv_full0 + 8 * stg, (j / STAGES) & 1, &s_abort, pp.wait_limit)) {
         fail(24);
         return false;
       }
@@ -610,7 +619,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       const int stg = j % STAGES;
       // the next tile's scores run while the row threads work on this tile's
       if (j + 1 < ntiles && !scores(j + 1)) break;
-      if (s_abort || !bar_wait(p_full, j & 1, &s_abort) || (j > 0 && !bar_wait(o_free, (j - 1) & 1, &s_abort))) {
+      if (s_abort || !bar_wait(p_full, j & 1, &s_abort, pp.wait_limit) || (j > 0 && !bar_wait(o_free, (j - 1) & 1, &s_abort, pp.wait_limit))) {
         fail(25);
         break;
       }
@@ -624,6 +633,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       mma_commit(o_full);
       mma_commit(kv_free0 + 8 * stg);
     }
+    // nobody frees tensor memory under a product, also where this thread or another one gave up
+    mma_commit(idle);
+    bar_wait(idle, 0, nullptr, kWaitLimitP);
     }
   }
 
@@ -634,6 +646,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
   if (splits == 1) return;
+  // where a wait ran out, converters may have filled the rings over what the rows left there
+  if (s_abort && tid < kRowsP) s_stat[tid] = make_float2(0.f, NAN);
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int share = kRowsP / (int)splits, rows_here = min(pp.rows_per_tile, row_end - s_first);
   for (int i = tid; i < share * (HD / 4); i += kThreadsP) {
@@ -678,6 +692,7 @@ pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_k
   p.rows_per_tile = kRowsP / a.group;
   p.min_cols = min_cols;
   p.err_flag = ctx->dev_err;
+  p.wait_limit = ctx->kv8_wait_limit ? ctx->kv8_wait_limit : kWaitLimitP;
   // tiles of rows: each sequence ends with one that may not be full
   const long long full = ((long long)a.n_rows + p.rows_per_tile - 1) / p.rows_per_tile, most = full + std::min(a.n_seqs - 1, a.n_rows - 1);
   PI_REQUIRE(ctx, most <= 65535, "%lld tiles of rows: at most 65535", most);
