@@ -575,8 +575,8 @@ pi_status pi_kv8_write(pi_ctx* ctx, pi_kv8_pool* pool, int layer, int dtype, con
  * h / (num_heads / num_kv_heads).  Weights are softmax(scale q k), accumulated in f32.  tables, lens, cu_rows and row_pos
  * of `arrays` are read (the others may be NULL), of its first n_seqs sequences; rows outside every sequence are not written.
  * max_seq_rows (most rows of one sequence) and max_context (the longest context) choose the kernel and how it is cut,
- * and with that the order of sums; results are right whatever they say.  At most 65535 sequences, and as many tiles of
- * 16 (row, query head) pairs of one KV head in a sequence.  out may be q itself.  Waits inside the kernels are bounded
+ * and with that the order of sums; results are right whatever they say.  At most 65535 sequences, and
+ * 2^31 - 2^21 (row, query head) pairs of one KV head.  out may be q itself.  Waits inside the kernels are bounded
  * (PI_OPT_KV8_WAIT_LIMIT): where one runs out the rows concerned become NaN and the next pi_ctx_synchronize returns
  * PI_ERR_TIMEOUT; a caller that never synchronises through the context sees the NaN alone. */
 pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int layer, int num_heads, int dtype, const void* q_dev, size_t q_stride,

@@ -57,7 +57,7 @@ struct pi_kv8_attn_params {
 };
 // Sequences of at most max_cols columns (rows times group), and those of more than min_cols.
 pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn_params& p, int max_seq_rows, int max_context, int max_cols);
-bool pi_kv8_prefill_takes(const pi_kv8_pool* pool, int group);
+bool pi_kv8_prefill_takes(const pi_kv8_pool* pool, const pi_kv8_attn_params& p);
 pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_kv8_attn_params& p, int min_cols, int max_context);
 
 // A launch on the context's stream that may begin while the kernel ahead of it ends (every kernel waits for that one before it touches

@@ -13,7 +13,6 @@ pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn
   const long long cols = (long long)max_seq_rows * p.group;
   const int nt = cols <= 8 ? 1 : 2, planes = p.dtype == PI_F32 ? 2 : 1;
   const long long col_tiles = (cols + 8 * nt - 1) / (8 * nt);
-  PI_REQUIRE(ctx, col_tiles <= 65535 && p.n_seqs <= 65535, "%lld column tiles of %d sequences: at most 65535 each", col_tiles, p.n_seqs);
   // The warps that work on one sequence's head: about as many as give every SM fourteen (what registers leave room for is sixteen), with
   // a round or more for each.  Up to eight are one CTA, more are clusters of CTAs of four, of eight where a cluster is full.
   // 64 sequences of 256 to 2048 tokens, 4 KV heads of 64: 21.5 us with 8 warps, 30 with 4, 27 with 16; 16 of 3000 to 4096, 8 of 128:
@@ -25,7 +24,7 @@ pi_status pi_launch_kv8_decode(pi_ctx* ctx, const pi_kv8_pool* pool, pi_kv8_attn
   while (n < kMaxSplit * kMaxWarps && base * n * 2 <= 16 * ctx->sm_count && rounds >= n * 2) n *= 2;
   const int splits = n <= kMaxWarps ? 1 : (int)std::min<long long>(kMaxSplit, n / 4), warps = (int)(n / splits);
   p.by_workers = pi_divisor(splits * warps);
-  const dim3 grid((unsigned)(p.kv_heads * splits), (unsigned)p.n_seqs, (unsigned)col_tiles);
+  const dim3 grid((unsigned)(p.kv_heads * splits), (unsigned)p.n_seqs, (unsigned)std::min<long long>(col_tiles, 65535));   // its CTAs go on to the columns behind
   switch (pool->pitch) {
     case 32: return launch_decode_pitch<32>(ctx, pool->kind, planes, nt, p, grid, splits, warps);
     case 64: return launch_decode_pitch<64>(ctx, pool->kind, planes, nt, p, grid, splits, warps);
@@ -45,12 +44,13 @@ extern "C" pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int 
   PI_REQUIRE(ctx, num_heads > 0 && num_heads % L.num_kv_heads == 0, "%d query heads do not divide into %d KV heads", num_heads, L.num_kv_heads);
   PI_REQUIRE(ctx, dtype == PI_F32 || dtype == PI_BF16 || dtype == PI_F16, "queries of kind %d: PI_F32, PI_BF16 or PI_F16 are wanted", dtype);
   PI_REQUIRE(ctx, n_rows >= 0 && n_seqs >= 0, "negative row or sequence count");
+  PI_REQUIRE(ctx, n_seqs <= 65535, "%d sequences: at most 65535", n_seqs);
   if (n_rows == 0 || n_seqs == 0) return PI_OK;
   PI_REQUIRE(ctx, q_dev && out_dev && a->tables && a->lens && a->cu_rows && a->row_pos, "null pointer");
   PI_REQUIRE(ctx, a->block_size == L.block_size, "the step's blocks hold %d tokens, the pool's %d", a->block_size, L.block_size);
   PI_REQUIRE(ctx, a->max_blocks > 0 && n_seqs <= a->max_seqs && n_rows <= a->max_rows, "%d sequences and %d rows: the step's arrays have room for %d and %d", n_seqs, n_rows,
              a->max_seqs, a->max_rows);
-  PI_REQUIRE(ctx, (long long)n_rows * num_heads / L.num_kv_heads <= 0x7fffffffll - 4096, "%d rows of %d query heads are too many", n_rows, num_heads);
+  PI_REQUIRE(ctx, (long long)n_rows * num_heads / L.num_kv_heads <= 0x7fffffffll - (1 << 21), "%d rows of %d query heads are too many", n_rows, num_heads);
   PI_REQUIRE(ctx, (long long)a->max_blocks * L.block_size <= 0x7fffffffll - 4096, "tables of %d blocks of %d tokens reach beyond position 2^31", a->max_blocks, L.block_size);
   const size_t row = (size_t)num_heads * L.head_dim, size = dtype == PI_F32 ? 4 : 2;
   PI_REQUIRE(ctx, (q_stride >= row && out_stride >= row) || n_rows == 1, "rows of %zu values cannot be %zu (queries) and %zu (results) apart", row, q_stride, out_stride);
@@ -93,7 +93,7 @@ extern "C" pi_status pi_kv8_attention(pi_ctx* ctx, const pi_kv8_pool* pool, int 
   // Sequences of up to 64 columns beside longer portions: each kernel takes its own, whatever the lengths on the device are.  A sequence
   // alone is a portion.  4096 positions, 8 KV heads of 128: 4 sequences of 32 columns take 37 us on the one kernel and 94 on the other, one
   // of 128 columns 34 and 35.
-  if ((long long)max_seq_rows * p.group <= kFewColumns || !pi_kv8_prefill_takes(pool, p.group)) return pi_launch_kv8_decode(ctx, pool, p, max_seq_rows, max_context, 0x7fffffff);
+  if ((long long)max_seq_rows * p.group <= kFewColumns || !pi_kv8_prefill_takes(pool, p)) return pi_launch_kv8_decode(ctx, pool, p, max_seq_rows, max_context, 0x7fffffff);
   if (n_seqs == 1) return pi_launch_kv8_prefill(ctx, pool, p, 0, max_context);
   if (p.group <= kFewColumns) PI_TRY(pi_launch_kv8_decode(ctx, pool, p, kFewColumns / p.group, max_context, kFewColumns));
   return pi_launch_kv8_prefill(ctx, pool, p, p.group <= kFewColumns ? kFewColumns : 0, max_context);

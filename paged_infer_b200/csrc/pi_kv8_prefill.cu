@@ -38,7 +38,7 @@ namespace {
 
 using namespace pi_kv8;
 
-constexpr int kRowsP = 128, kPartP = 64, kThreadsP = 20 * 32, kMostStages = 4;   // a part: the tokens of a tile that four warps widen
+constexpr int kRowsP = 128, kPartP = 64, kThreadsP = 20 * 32, kMostStages = 4, kMostSplitsP = 8;   // a part: the tokens of a tile that four warps widen
 constexpr long long kWaitLimitP = 1ll << 31;   // clocks of a wait: about a second
 
 struct PrefillParams {
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   uint32_t split, splits;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
-  const int kvh = blockIdx.x / splits;
+  const int row_tile = (int)(blockIdx.x / splits) / p.kv_heads, kvh = (int)(blockIdx.x / splits) - row_tile * p.kv_heads;
   const uint32_t kv_full0 = s_u32(&bars[0]), kv_free0 = s_u32(&bars[kMostStages]), s_full0 = s_u32(&bars[2 * kMostStages]), p_full = s_u32(&bars[2 * kMostStages + 2]),
                  o_full = s_u32(&bars[2 * kMostStages + 3]), o_free = s_u32(&bars[2 * kMostStages + 4]), idle = s_u32(&bars[2 * kMostStages + 5]);
   pi_grid_dependency_wait_only();
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         const int t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
       }
-      const int y = (int)blockIdx.y - ahead;
+      const int y = row_tile - ahead;
       const unsigned hit = __ballot_sync(0xffffffffu, y < upto && y >= upto - tiles);
       if (hit) {
         const int at = __ffs(hit) - 1;
@@ -684,7 +684,15 @@ pi_status launch_prefill(pi_ctx* ctx, const PrefillParams& p, dim3 grid, int spl
 
 }  // namespace
 
-bool pi_kv8_prefill_takes(const pi_kv8_pool* pool, int group) { return (pool->pitch == 64 || pool->pitch == 128) && group <= kRowsP; }
+// Tiles of rows: each sequence ends with one that may not be full.
+static long long prefill_tiles(const pi_kv8_attn_params& a) {
+  const int rows = kRowsP / a.group;
+  return ((long long)a.n_rows + rows - 1) / rows + std::min(a.n_seqs - 1, a.n_rows - 1);
+}
+
+bool pi_kv8_prefill_takes(const pi_kv8_pool* pool, const pi_kv8_attn_params& a) {
+  return (pool->pitch == 64 || pool->pitch == 128) && a.group <= kRowsP && prefill_tiles(a) * a.kv_heads <= 0x7fffffffll / kMostSplitsP;   // CTAs of a grid
+}
 
 pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_kv8_attn_params& a, int min_cols, int max_context) {
   PrefillParams p = {};
@@ -693,14 +701,12 @@ pi_status pi_launch_kv8_prefill(pi_ctx* ctx, const pi_kv8_pool* pool, const pi_k
   p.min_cols = min_cols;
   p.err_flag = ctx->dev_err;
   p.wait_limit = ctx->kv8_wait_limit ? ctx->kv8_wait_limit : kWaitLimitP;
-  // tiles of rows: each sequence ends with one that may not be full
-  const long long full = ((long long)a.n_rows + p.rows_per_tile - 1) / p.rows_per_tile, most = full + std::min(a.n_seqs - 1, a.n_rows - 1);
-  PI_REQUIRE(ctx, most <= 65535, "%lld tiles of rows: at most 65535", most);
+  const long long full = ((long long)a.n_rows + p.rows_per_tile - 1) / p.rows_per_tile;
   // few tiles share their positions out among clusters, four tiles of them or more to a CTA
   const long long seen = a.window > 0 ? std::min<long long>(max_context, (long long)a.window + a.n_rows) : max_context;
   int splits = 1;
-  while (splits < 8 && full * a.kv_heads * splits * 2 <= ctx->sm_count && seen / 64 >= 8 * splits * 2) splits *= 2;
-  const dim3 grid((unsigned)(a.kv_heads * splits), (unsigned)most);
+  while (splits < kMostSplitsP && full * a.kv_heads * splits * 2 <= ctx->sm_count && seen / 64 >= 8 * splits * 2) splits *= 2;
+  const dim3 grid((unsigned)(prefill_tiles(a) * a.kv_heads * splits));   // a tile's heads side by side, a head's CTAs a cluster
   const bool two = a.dtype == PI_F32;
   if (pool->kind == PI_INT8) {
     if (pool->pitch == 64) return two ? launch_prefill<PI_INT8, 64, 2>(ctx, p, grid, splits) : launch_prefill<PI_INT8, 64, 1>(ctx, p, grid, splits);

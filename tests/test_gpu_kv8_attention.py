@@ -3,8 +3,9 @@ import numpy as np
 import pytest
 import torch
 
+from kv8_helpers import attention_reference, attention_tolerance
 from paged_infer_b200 import _lib, api
-from test_gpu_kv8 import attention_case
+from test_gpu_kv8 import attention_case, i32, new_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,51 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_nan(ctx, dtype, heads, kv_h
     assert torch.equal(again, out)
     with pytest.raises(api.PiError):
         ctx.set_option(_lib.PI_OPT_KV8_WAIT_LIMIT, -1)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,news", [(128, 1, 64, [40000, 30000]), (64, 1, 64, [100000, 1, 39999]), (200, 1, 24, [6000])])
+def test_attention_of_more_tiles_than_a_grid_has_rows(ctx, heads, kv_heads, dim, news):
+    """Groups so wide that a tile holds one or two rows, in batches of more than 65535 tiles; and more tiles of columns than that in one
+    sequence.  Rows here and there against the reference, all of them against the call that is told to expect few."""
+    block, window = 16, 20
+    contexts = np.array(news)
+    rng = np.random.default_rng(heads)
+    after = -(-contexts // block)
+    wide, blocks = int(after.max()), int(after.sum())
+    tables, at = np.full((len(news), wide), -1, np.int32), 0
+    for b, n in enumerate(after):
+        tables[b, :n] = np.arange(at, at + n)
+        at += n
+    cu = np.concatenate([[0], np.cumsum(news)])
+    rows, pos = int(cu[-1]), np.concatenate([np.arange(n) for n in news])
+    cache = new_cache(ctx, "int8", 1, blocks, kv_heads, block, dim, seed=1)
+    g = torch.Generator(device="cuda").manual_seed(heads)
+    q = torch.randn(rows, heads, dim, generator=g, device="cuda", dtype=torch.bfloat16)
+    plan = api.StepPlan(ctx, block, i32(tables), lens=i32(after), cu_rows=i32(cu), row_pos=i32(pos))
+    a, out, again = api.PagedAttention8(cache.layout, heads), torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    a.run_device(q, out, cache, plan, window=window)
+    ctx.synchronize()
+    a.run_device(q, again, cache, plan, window=window, max_seq_rows=1)
+    some = np.unique(np.concatenate([cu[:-1], cu[1:] - 1, rng.integers(0, rows, 40), [65535, 65536, rows - 2] if rows > 65536 else []]).astype(int))
+    seq = np.searchsorted(cu, some, side="right") - 1
+    codes, scales = cache.codes[0].view(torch.uint8).cpu().numpy(), cache.scales[0].cpu().numpy()
+    sub = np.concatenate([[0], np.cumsum([(seq == b).sum() for b in range(len(news))])])
+    want, most, mass = attention_reference(q[some].float().cpu().numpy(), codes, scales, tables=tables, lens=after, cu=sub, pos=pos[some], block=block, kind="int8", window=window)
+    tolerance = attention_tolerance(want, most, mass, dim, "bf16")
+    for o in (out, again):
+        assert (np.abs(o[some].float().cpu().numpy() - want) <= tolerance).all()
+    # a rounding of the result each, and 2^-9 of the largest value: 2^-10 of the weights and, scores being products of 64 channels at most
+    # (the sum of their magnitudes below 25), 4 x 25 x 78 x 2^-23 from those
+    off = (out.float() - again.float()).abs() - 2.0 ** -7 * torch.maximum(out.float().abs(), again.float().abs())
+    assert off.max() <= 2 * 2.0 ** -9 * 100 * 0.025      # largest |code| x largest scale of the cache
+
+
+def test_a_refused_call_leaves_the_results_alone(ctx):
+    q, out, cache, plan, given = attention_case(ctx, "int8", "bf16", 16, 8, 2, 64, [300, 40], [130, 1], seed=3)
+    n = 65536
+    many = api.StepPlan(ctx, 16, i32(np.full((n, 1), -1)), lens=i32(np.zeros(n)), cu_rows=i32(np.minimum(np.arange(n + 1), 131)), row_pos=plan.row_pos)
+    before = out.clone()
+    with pytest.raises(api.PiError, match="65535"):
+        api.PagedAttention8(cache.layout, 8).run_device(q, out, cache, many, layer=1)
+    ctx.synchronize()
+    assert torch.equal(out, before)
