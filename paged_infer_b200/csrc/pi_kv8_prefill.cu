@@ -7,7 +7,8 @@
 //     scores  S = Q K^T        A = Q (written once),  B = codes of K, [token][channel]
 //     output  O = P V          A = P,                 B = codes of V transposed, [channel][token]
 // A row's thread multiplies the K scale in as it reads its scores, and weighs exp(score) by V scale / r, r a power of two above the
-// V scales that the row sees in the tile, so that P stays in f16's range whatever the scales are; the product of a tile is read
+// largest product of weight and V scale in the tile, so that P stays in f16's range whatever the scales are, and what a large scale
+// takes from a small one's bits it takes by what it adds to the result; the product of a tile is read
 // back, multiplied by r and added to the row's f32 output in registers.  The running maximum may lag 2^8 behind, so that the output
 // is hardly ever rescaled.
 //
@@ -52,10 +53,9 @@ struct PrefillParams {
 struct Group {
   int base, valid;
   float k_scale;
-  int v_exp;
-  float v_log;
+  float v_exp, v_log;
 };
-constexpr int kNoScale = -100000;   // v_exp of a zero scale
+constexpr float kNoScale = -100000.f;   // v_exp of a zero scale
 
 __device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void st_shared(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
   __shared__ Group s_group[kMostStages][8];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ float s_most[2][2][kRowsP];   // [tile parity][half][row]
+  __shared__ float2 s_most[2][2][kRowsP];   // [tile parity][half][row]
   __shared__ int s_lo, s_hi, s_seq, s_first;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = p.block_size, G = p.group;
@@ -344,30 +344,25 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       constexpr int COLS = TILE / 2, GROUPS = COLS / 16;   // of this thread
       const uint32_t s_col = lane_addr + L::col_s + buf * TILE + half * COLS;
       // the tile as a whole: lane g looks at group g
-      int v_top, lowest, highest;
+      int lowest, highest;
       bool filled;
       {
-        const bool there = lane < 2 * GROUPS;
-        const Group q = group[there ? lane : 0];
-        v_top = __reduce_max_sync(0xffffffffu, there ? q.v_exp : kNoScale);
+        const Group q = group[lane < 2 * GROUPS ? lane : 0];
         lowest = __reduce_min_sync(0xffffffffu, q.base);
         highest = __reduce_max_sync(0xffffffffu, q.base + 15);
         filled = __all_sync(0xffffffffu, q.valid == 16);
       }
       const bool masks = !__all_sync(0xffffffffu, filled && from <= lowest && to >= highest);
-      // where not all of it is seen: a bit per column of this thread's groups; r goes by what the row sees
+      // where not all of it is seen: a bit per column of this thread's groups
       uint32_t seen[GROUPS];
       if (masks) {
-        v_top = kNoScale;
 #pragma unroll
-        for (int g = 0; g < 2 * GROUPS; ++g) {
-          const Group q = group[g];
+        for (int g = 0; g < GROUPS; ++g) {
+          const Group q = group[half * GROUPS + g];
           const int f = max(0, from - q.base), l = min(to - q.base, q.valid - 1);
-          if (f <= l) v_top = max(v_top, q.v_exp);
-          if (g / GROUPS == half) seen[g % GROUPS] = f <= l ? (0xffffu >> (15 - l)) & (0xffffu << f) : 0;
+          seen[g] = f <= l ? (0xffffu >> (15 - l)) & (0xffffu << f) : 0;
         }
       }
-      const int v_unit = v_top == kNoScale ? 0 : min(v_top + 1, 126);   // r = 2^v_unit
       float w[COLS];
       {
         uint32_t raw[COLS];
@@ -377,8 +372,8 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 #pragma unroll
         for (int i = 0; i < COLS; ++i) w[i] = __uint_as_float(raw[i]);
       }
-      // the largest score of the tile
-      float most = -INFINITY;
+      // the largest score of the tile, and of score and V scale together
+      float most = -INFINITY, reach = -INFINITY;
       if (masks) {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
@@ -392,12 +387,20 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 #pragma unroll
         for (int i = 0; i < 16; ++i) top2[i & 1] = fmaxf(top2[i & 1], w[g * 16 + i]);
         const float t = fmaxf(top2[0], top2[1]);
-        if (t > -INFINITY) most = fmaxf(most, t * (factor * group[half * GROUPS + g].k_scale));
+        if (t > -INFINITY) {
+          const float score = t * (factor * group[half * GROUPS + g].k_scale);
+          most = fmaxf(most, score);
+          reach = fmaxf(reach, score + group[half * GROUPS + g].v_exp);
+        }
       }
-      // the other half's; both threads come to the same maximum
-      s_most[buf][half][m] = most;
+      // the other half's; both threads come to the same maxima
+      s_most[buf][half][m] = make_float2(most, reach);
       meet();
-      most = fmaxf(most, s_most[buf][half ^ 1][m]);
+      {
+        const float2 other = s_most[buf][half ^ 1][m];
+        most = fmaxf(most, other.x);
+        reach = fmaxf(reach, other.y);
+      }
       float keep = 1.f;
       if (most > top + kLag) {
         keep = top == -INFINITY ? 1.f : exp2_fast(top - most);
@@ -405,14 +408,17 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
       }
       sum *= keep;
       const float base = (top == -INFINITY ? 0.f : top) - kTopWeight;
+      // r = 2^v_unit: a weight relative to 2^kTopWeight times its V scale is below it.  Where all that the row sees has V scales or weights of next to
+      // nothing, r stays a normal number.
+      const float v_unit = fminf(fmaxf(ceilf(reach - (base + kTopWeight)) + 1.f, -126.f), 127.f);
       uint32_t hi[COLS / 2], lo[PLANES == 2 ? COLS / 2 : 1];
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         const Group q = group[half * GROUPS + g];
         const float f = factor * q.k_scale;
         // weights times V scale / r; a zero scale's codes are zero, so that any factor does
-        float shift = q.v_exp == kNoScale ? 0.f : (float)(q.v_exp - v_unit) + q.v_log;
-        if (shift < -100.f) shift = -100.f;   // 2^-100 of what the row sees beside it; not a number stays that
+        float shift = q.v_exp == kNoScale ? 0.f : q.v_exp - v_unit + q.v_log;
+        if (shift < -100.f) shift = -100.f;   // 2^-100 of the largest in the tile; not a number stays that
         const float less = shift - base;
         float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         continue;
       }
       fold_keep = keep;
-      fold_unit = exp2_fast((float)v_unit);
+      fold_unit = exp2_fast(v_unit);
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         t_st8(lane_addr + L::col_p + half * (COLS / 2) + g * 8, hi + g * 8);
@@ -450,9 +456,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
     if (alive && ntiles > 0) alive = fold(ntiles - 1);
     if (!alive) sum = NAN;   // a wait ran out: the row's results say so, whatever CTA they come from
     // the halves' sums, in the buffer that the last tile did not use
-    s_most[ntiles & 1][half][m] = sum;
+    s_most[ntiles & 1][half][m].x = sum;
     meet();
-    sum = s_most[ntiles & 1][0][m] + s_most[ntiles & 1][1][m];
+    sum = s_most[ntiles & 1][0][m].x + s_most[ntiles & 1][1][m].x;
     if (splits == 1) {
       if (live) {
 #pragma unroll
@@ -553,7 +559,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         const float sv = cur.k_scales.y;
         int e = 0;
         const float mant = frexpf(sv, &e);   // [0.5, 1)
-        q.v_exp = sv == 0.f ? kNoScale : e - 1;
+        q.v_exp = sv == 0.f ? kNoScale : (float)(e - 1);
         q.v_log = sv == 0.f ? 0.f : (sv < INFINITY ? log2f(2.f * mant) : NAN);
         s_group[stg][part * 4 + cw] = q;
       }

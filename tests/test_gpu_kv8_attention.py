@@ -1,9 +1,11 @@
 """Attention over the 8-bit cache where its parts meet: waits that run out, dispatch of large batches, scales far apart, both planes."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
-from kv8_helpers import attention_reference, attention_tolerance
+from kv8_helpers import TORCH, TYPES, attention_reference, attention_tolerance
 from paged_infer_b200 import _lib, api
 from test_gpu_kv8 import attention_case, i32, new_cache
 
@@ -86,3 +88,73 @@ def test_a_refused_call_leaves_the_results_alone(ctx):
         api.PagedAttention8(cache.layout, 8).run_device(q, out, cache, many, layer=1)
     ctx.synchronize()
     assert torch.equal(out, before)
+
+
+def weighted_reference(q, codes, scales, table, pos, block, kind, window=0):
+    """(out, sum of weight x largest |v| of the token, largest sum of |q||k| scale) of one sequence in 64 bits; codes as values of one layer."""
+    rows, heads, dim = q.shape
+    group = heads // codes.shape[1]
+    n = int(pos.max()) + 1
+    t = np.arange(n)
+    value = codes[table[t // block], :, :, t % block, :dim].astype(np.float64) * scales[table[t // block]].astype(np.float64)[..., None]   # [n][kv_heads][2][dim]
+    out, weighed, mass = np.zeros((rows, heads, dim)), np.zeros((rows, heads)), np.zeros((rows, heads))
+    for h in range(heads):
+        k, v = value[:, h // group, 0], value[:, h // group, 1]
+        s = q[:, h].astype(np.float64) @ k.T * dim ** -0.5
+        unseen = (t[None] > pos[:, None]) | ((t[None] <= pos[:, None] - window) if window else False)
+        s[unseen] = -np.inf
+        w = np.exp(s - s.max(1, keepdims=True))
+        w /= w.sum(1, keepdims=True)
+        out[:, h], weighed[:, h] = w @ v, w @ np.abs(v).max(1)
+        mass[:, h] = np.where(unseen, 0, np.abs(q[:, h]).astype(np.float64) @ np.abs(k).T * dim ** -0.5).max(1)
+    return out, weighed, mass
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim,news,context", [(64, 200, 300), (128, 200, 300), (64, 1, 300), (128, 40, 2500)])
+@pytest.mark.parametrize("ratio", [24, 40, -30])
+def test_a_large_scale_of_next_to_no_weight(ctx, kind, dtype, dim, news, context, ratio):
+    """Blocks whose V scale is 2^ratio of their neighbours', seen with a weight so small that they add little: every result keeps its
+    precision relative to what it is made of, sum of weight x |v|, not to the largest |v| in sight.  The last case but one: single
+    tokens; the last: a cluster shares the positions."""
+    rng = np.random.default_rng(ratio + 50 + dim)
+    block, heads, kv_heads = 16, 4, 2
+    blocks = -(-context // block)
+    shape = (2, blocks, kv_heads, 2, block, dim)
+    values = np.clip(np.round(rng.standard_normal(shape) * 30), -60, 60).astype(np.float32)
+    if kind == "e4m3":
+        values = torch.tensor(values).to(torch.float8_e4m3fn).float().numpy()
+    scales = (np.exp(rng.standard_normal(shape[:4]) * 0.2) / 40).astype(np.float32)
+    q = rng.standard_normal((news, heads, dim)).astype(np.float32)
+    q[..., 0] = 8.0
+    values[..., 0, :, 0] = 0                              # K's first channel: nothing, but in the blocks in question
+    odd = np.arange(2, blocks, 5)
+    far = 2.0 ** abs(ratio)
+    # weights of about exp(-ratio ln 2 - 10) at 2^ratio, of 1 at 2^-ratio (the others then lie that far below)
+    low = (max(ratio, 0) * math.log(2) + 10) * dim ** 0.5 / 8.0 / 60 if ratio > 0 else 0.0
+    if ratio > 0:
+        values[1][odd, :, 0] = 0
+        values[1][odd, :, 0, :, 0] = -60
+        scales[1][odd, :, 0] = low
+        scales[1][odd, :, 1] *= far
+    else:
+        values[1][odd, :, 0] = 0
+        values[1][odd, :, 0, :, 0] = 60
+        scales[1][odd, :, 0] = (abs(ratio) * math.log(2) + 10) * dim ** 0.5 / 8.0 / 60
+        scales[1][odd, :, 1] /= far
+    table = rng.permutation(blocks)
+    place = np.empty(blocks, int)
+    place[table] = np.arange(blocks)
+    codes = torch.tensor(values, device="cuda").to(TORCH[kind])
+    layout = api.KvLayout(2, blocks, block, kv_heads, dim)
+    cache = api.KvCache8(ctx, layout, codes=codes, scales=torch.tensor(scales, device="cuda"))
+    qt = torch.tensor(q, device="cuda").to(TYPES[dtype])
+    out = torch.full_like(qt, 7.0)
+    pos = np.arange(context - news, context)
+    plan = api.StepPlan(ctx, block, i32(table[None]), lens=i32([blocks]), cu_rows=i32([0, news]), row_pos=i32(pos))
+    api.PagedAttention8(layout, heads).run_device(qt, out, cache, plan, layer=1)
+    want, weighed, mass = weighted_reference(qt.float().cpu().numpy(), values[1], scales[1], table, pos, block, kind)
+    tolerance = attention_tolerance(want, weighed, mass, dim, dtype) + (2.0 ** -25 if dtype == "f16" else 0)   # half of f16's smallest step
+    off = np.abs(out.float().cpu().numpy() - want) - tolerance
+    assert not (off > 0).any(), off.max()
