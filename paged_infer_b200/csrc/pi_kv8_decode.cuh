@@ -6,16 +6,18 @@
 //     S^T[16 tokens][8 columns] = K q^T,    O^T[dims][8 columns] += scale_v (V^T P^T),    a column = one query head of one row.
 // A group of eight query heads fills a product; four need no more of them than eight would.  f32 queries, and the weights of f32
 // outputs, are two f16 planes (22 bits); those of bf16 and f16 outputs are one.  Queries are brought to [-1, 1] by a power of two
-// per column, weights to 2^14 at most, so that neither leaves f16's normal range; the scales stay in f32.
+// per column, weights to 2^15 at most, so that neither leaves f16's normal range; the scales stay in f32.
 //
 // Codes go from memory straight to the registers that feed the products: the k index of a product may be permuted at will, so a
 // lane takes whole words of a token's codes for K, and, for V, of the four tokens whose weights it holds; pairs of tokens are put
 // together by byte permutes.  The next tile's K codes are requested as soon as this tile's are used up, its V codes likewise, so that
 // every warp has loads under way all the time without a second set of registers and without shared memory.
 //
-// int8 codes become f16 by a byte permute into the mantissa of 1024 (1024 + 128 + code).  With two planes the 1152 is subtracted from
-// every pair.  With one plane it stays in and the accumulators start from -1152 times the sum of the other operand instead: the sums
-// are 33 times larger than without, which costs 5 of the accumulator's 24 bits where the result has 8 or 11.
+// int8 codes become f16 by a byte permute into the mantissa of 1024 (1024 + 128 + code), and 1152 is subtracted from every pair.  Only
+// V's, with one plane, keep it, and the accumulators start from -1152 times the sum of the weights instead: a result is off by up to
+// 1152 x 2^-23 of its V scale for that, 2^-13 of a step of the codes.  Not K's: a score would be off by as much for every unit of the query,
+// which is a lot beside a channel of large codes in which the query is small, where the other codes are few steps (a tenth of a weight
+// at 256 channels).  (One context of 131072: 108 us, 104 with K's left in; 16 of 3000 to 4096, int8: 32.1 and 31.4.)
 //
 // The tokens of a sequence are dealt to the warps of a CTA and to the CTAs of a cluster; partial results are joined through shared
 // memory, then through the cluster's: no scratch in device memory, and the order of the sums is fixed.
@@ -83,7 +85,7 @@ struct Shape {
   static constexpr int TT = PITCH <= 64 && NT == 1 ? 2 : 1, min_ctas = PITCH <= 128 && NT == 1 ? 2 : 1, cols = 8 * NT;
   static constexpr int line = PITCH + 4;   // floats between columns where warps meet
 };
-// Shared memory: query fragments, per column (first and last position seen, factor, bias), (max, sum) per warp, per CTA, partial results.
+// Shared memory: query fragments, per column (first and last position seen, factor), (max, sum) per warp, per CTA, partial results.
 template <int PITCH, int PLANES, int NT>
 struct Layout {
   static constexpr int cols = 8 * NT;
@@ -103,8 +105,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
   int* s_lo = reinterpret_cast<int*>(smem + Layout<PITCH, PLANES, NT>::queries);
   int* s_hi = s_lo + COLS;
   float* s_factor = reinterpret_cast<float*>(s_hi + COLS);
-  float* s_bias = s_factor + COLS;
-  float2* s_stat = reinterpret_cast<float2*>(s_bias + COLS);   // of the CTA
+  float2* s_stat = reinterpret_cast<float2*>(s_factor + 2 * COLS);   // of the CTA
   float2* s_warp = s_stat + COLS;                              // [warp][column]
   float* s_out = reinterpret_cast<float*>(s_warp + warps * COLS);   // [column][line] of the CTA
   float* s_part = s_out + COLS * LINE;                         // [warp][column][line]
@@ -239,7 +240,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
       // 2^(e - 127) <= most < 2^(e - 126); both powers below stay normal
       const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);
       const float shrink = __uint_as_float((253u - e) << 23);   // 2^(126 - e)
-      float bias = 0.f;
 #pragma unroll
       for (int i = 0; i < PITCH / 32; ++i) {
         const int d = 4 * (l8 + 8 * i), piece = d / (G::KB * 4), in = d % (G::KB * 4), to = (piece * (G::KB / 4) + in % G::KB / 4) * PLANES;
@@ -250,26 +250,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
         uint2* frag = reinterpret_cast<uint2*>(s_queries) + ((size_t)to * NT + c / 8) * 32 + (c % 8) * 4 + in / G::KB;
         frag[0] = hi;
         if constexpr (PLANES == 2) frag[NT * 32] = make_uint2(pack_rest(y[0], y[1], hi.x), pack_rest(y[2], y[3], hi.y));
-        if constexpr (BIASED) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-          bias += (a.x + a.y) + (b.x + b.y);
-        }
-      }
-      if constexpr (BIASED) {
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) bias += __shfl_xor_sync(0xffffffffu, bias, o);
       }
       if (l8 == 0) {
         const int pos = live ? p.row_pos[row] : -1;
         s_lo[c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         s_hi[c] = pos;
         s_factor[c] = __uint_as_float((e + 1) << 23) * p.scale2;   // 2^(e - 126)
-        s_bias[c] = -kBias * bias;
       }
     }
     __syncthreads();
 
-    float out[NT][G::mtiles][4], top[NT][2], sum[NT][2], factor[NT][2], q_bias[NT][2];
+    float out[NT][G::mtiles][4], top[NT][2], sum[NT][2], factor[NT][2];
     int lo[NT][2], hi[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -279,7 +270,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
         top[n][e] = -INFINITY;
         sum[n][e] = 0.f;
         factor[n][e] = s_factor[c];
-        q_bias[n][e] = BIASED ? s_bias[c] : 0.f;
         lo[n][e] = s_lo[c];
         hi[n][e] = min(s_hi[c], hi_all);
       }
@@ -321,10 +311,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
 #pragma unroll
         for (int e = 0; e < TT; ++e) {
           const uint32_t w0 = unsign<KIND>(kw[e][0][j]), w1 = unsign<KIND>(kw[e][1][j]);
-          a[e][0] = widen<KIND, BIASED>(w0, false);
-          a[e][1] = widen<KIND, BIASED>(w1, false);
-          a[e][2] = widen<KIND, BIASED>(w0, true);
-          a[e][3] = widen<KIND, BIASED>(w1, true);
+          a[e][0] = widen<KIND, false>(w0, false);
+          a[e][1] = widen<KIND, false>(w1, false);
+          a[e][2] = widen<KIND, false>(w0, true);
+          a[e][3] = widen<KIND, false>(w1, true);
         }
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl)
@@ -333,7 +323,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
             const uint2 b = reinterpret_cast<const uint2*>(s_queries)[((j * PLANES + pl) * NT + n) * 32 + lane];
 #pragma unroll
             for (int e = 0; e < TT; ++e) {
-              if (j == 0 && pl == 0) mma_f16_from(s[e][n], a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y, q_bias[n][0], q_bias[n][1]);
+              if (j == 0 && pl == 0) mma_f16_from(s[e][n], a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y, 0.f, 0.f);
               else mma_f16(s[e][n], a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y);
             }
           }

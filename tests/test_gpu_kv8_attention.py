@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from kv8_helpers import TORCH, TYPES, attention_reference, attention_tolerance
+from kv8_helpers import TORCH, TYPES, attention_reference, attention_tolerance, pitch_of
 from paged_infer_b200 import _lib, api
 from test_gpu_kv8 import attention_case, i32, new_cache
 
@@ -144,8 +144,6 @@ def test_a_large_scale_of_next_to_no_weight(ctx, kind, dtype, dim, news, context
         scales[1][odd, :, 0] = (abs(ratio) * math.log(2) + 10) * dim ** 0.5 / 8.0 / 60
         scales[1][odd, :, 1] /= far
     table = rng.permutation(blocks)
-    place = np.empty(blocks, int)
-    place[table] = np.arange(blocks)
     codes = torch.tensor(values, device="cuda").to(TORCH[kind])
     layout = api.KvLayout(2, blocks, block, kv_heads, dim)
     cache = api.KvCache8(ctx, layout, codes=codes, scales=torch.tensor(scales, device="cuda"))
@@ -158,3 +156,32 @@ def test_a_large_scale_of_next_to_no_weight(ctx, kind, dtype, dim, news, context
     tolerance = attention_tolerance(want, weighed, mass, dim, dtype) + (2.0 ** -25 if dtype == "f16" else 0)   # half of f16's smallest step
     off = np.abs(out.float().cpu().numpy() - want) - tolerance
     assert not (off > 0).any(), off.max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim,news", [(64, 1), (128, 1), (96, 3), (256, 2), (64, 60), (128, 60)])
+def test_an_outlier_channel_of_keys_beside_small_codes(ctx, dtype, dim, news):
+    """A K channel that sets the scale and in which the query is zero: a token's other codes are zero but for two of them, and scores keep
+    their precision relative to those, however large the query is beside the others."""
+    rng = np.random.default_rng(dim + news)
+    block, heads, kv_heads, context = 16, 8, 2, 70
+    blocks = -(-context // block)
+    shape = (2, blocks, kv_heads, 2, block, pitch_of(dim))
+    values = np.clip(np.round(rng.standard_normal(shape) * 35), -127, 127).astype(np.float32)
+    values[..., dim:] = 0
+    values[..., 0, :, :] = 0
+    np.put_along_axis(values[..., 0, :, :], rng.integers(1, dim, shape[:3] + (block, 2)), 1.0, -1)
+    values[..., 0, :, 0] = 127
+    scales = np.full(shape[:4], 1 / 40, np.float32)
+    scales[..., 0] = 3 * dim ** 0.5                       # scores of 1.5 to 6
+    q = torch.tensor(rng.uniform(0.5, 1.0, (news, heads, dim)), device="cuda").to(TYPES[dtype])
+    q[..., 0] = 0
+    table, pos = rng.permutation(blocks), np.arange(context - news, context)
+    layout = api.KvLayout(2, blocks, block, kv_heads, dim)
+    cache = api.KvCache8(ctx, layout, codes=torch.tensor(values, device="cuda").to(torch.int8), scales=torch.tensor(scales, device="cuda"))
+    plan = api.StepPlan(ctx, block, i32(table[None]), lens=i32([blocks]), cu_rows=i32([0, news]), row_pos=i32(pos))
+    out = torch.full_like(q, 7.0)
+    api.PagedAttention8(layout, heads).run_device(q, out, cache, plan, layer=1)
+    want, weighed, mass = weighted_reference(q.float().cpu().numpy(), values[1], scales[1], table, pos, block, "int8")
+    off = np.abs(out.float().cpu().numpy() - want) - attention_tolerance(want, weighed, mass, dim, dtype)
+    assert not (off > 0).any(), (off.max(), (off > 0).sum())
