@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from kv8_helpers import TORCH, TYPES, attention_reference, attention_tolerance, pitch_of
+from kv8_planes import plane_case, plane_reference, plane_tolerance
 from paged_infer_b200 import _lib, api
 from test_gpu_kv8 import attention_case, i32, new_cache
 
@@ -185,3 +186,29 @@ def test_an_outlier_channel_of_keys_beside_small_codes(ctx, dtype, dim, news):
     want, weighed, mass = weighted_reference(q.float().cpu().numpy(), values[1], scales[1], table, pos, block, "int8")
     off = np.abs(out.float().cpu().numpy() - want) - attention_tolerance(want, weighed, mass, dim, dtype)
     assert not (off > 0).any(), (off.max(), (off > 0).sum())
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("which", ["query", "weight"])
+@pytest.mark.parametrize("dim,heads,kv_heads,context,news", [(64, 8, 2, 40, 1), (128, 8, 2, 41, 2), (96, 4, 2, 40, 1), (256, 16, 1, 40, 1), (24, 4, 2, 33, 3), (64, 8, 1, 3000, 1), (128, 4, 1, 3000, 1),
+                                                               (64, 8, 2, 300, 200), (128, 8, 2, 300, 200), (64, 8, 1, 3000, 20), (128, 8, 1, 3000, 20), (96, 8, 2, 90, 40)])
+def test_f32_rows_have_both_planes(ctx, kind, which, dim, heads, kv_heads, context, news):
+    """Single tokens and portions, each alone and with the positions shared by a cluster."""
+    block = 16
+    q, values, k_scale, v_scale = plane_case(which, dim, context, news, heads, kv_heads)
+    blocks = -(-context // block)
+    codes = np.zeros((1, blocks * block, kv_heads, 2, pitch_of(dim)), np.float32)
+    codes[0, :context, ..., :dim] = values
+    codes = codes.reshape(1, blocks, block, kv_heads, 2, -1).transpose(0, 1, 3, 4, 2, 5)
+    scales = np.empty((1, blocks, kv_heads, 2), np.float32)
+    scales[..., 0], scales[..., 1] = k_scale, v_scale
+    layout = api.KvLayout(1, blocks, block, kv_heads, dim)
+    cache = api.KvCache8(ctx, layout, codes=torch.tensor(codes, device="cuda").to(TORCH[kind]).contiguous(), scales=torch.tensor(scales, device="cuda"))
+    pos = np.arange(context - news, context)
+    plan = api.StepPlan(ctx, block, i32(np.arange(blocks)[None]), lens=i32([blocks]), cu_rows=i32([0, news]), row_pos=i32(pos))
+    qt = torch.tensor(q, device="cuda")
+    out = torch.full_like(qt, 7.0)
+    api.PagedAttention8(layout, heads).run_device(qt, out, cache, plan)
+    want, weighed = plane_reference(q, values, k_scale, v_scale, pos)
+    off = np.abs(out.cpu().numpy() - want) - plane_tolerance(want, weighed)
+    assert not (off > 0).any(), off.max()
