@@ -212,3 +212,37 @@ def test_f32_rows_have_both_planes(ctx, kind, which, dim, heads, kv_heads, conte
     want, weighed = plane_reference(q, values, k_scale, v_scale, pos)
     off = np.abs(out.cpu().numpy() - want) - plane_tolerance(want, weighed)
     assert not (off > 0).any(), off.max()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,kv_heads,dim,contexts,news", [(4, 1, 256, [2526, 5000, 7021], [1, 1, 1]), (2, 1, 256, [366, 400, 622], [1, 2, 1]), (4, 2, 128, [339, 429], [1, 1]), (8, 2, 64, [700], [90]), (4, 2, 128, [1500], [90])])
+def test_f32_rows_against_64_bits_as_a_whole(ctx, kind, heads, kv_heads, dim, contexts, news):
+    """Results are sums of values of random signs, so that their error over their norm is the root mean square of the weights' relative
+    errors, below the sum of what those can be for scores of a few units: the exponential 2^-22, its argument (below 8) 2^-22 ln 2, the score's
+    factor and the queries' planes 2^-23 each; sums of products add nothing to speak of.  Together 2^-20.5."""
+    rng = np.random.default_rng(dim + len(news))
+    block, B = 16, len(news)
+    after = [-(-c // block) for c in contexts]
+    blocks, wide = sum(after), max(after)
+    shape = (1, blocks, kv_heads, 2, block, dim)
+    values = torch.tensor(np.clip(np.round(rng.standard_normal(shape) * 35), -127, 127), device="cuda", dtype=torch.float32)
+    codes = values.to(torch.int8) if kind == "int8" else (values * 3).to(torch.float8_e4m3fn)
+    scales = torch.tensor(np.exp(rng.standard_normal(shape[:4]) * 0.2) / (35 if kind == "int8" else 105), device="cuda", dtype=torch.float32)
+    tables, at = np.full((B, wide), -1), 0
+    for b, n in enumerate(after):
+        tables[b, :n] = np.arange(at, at + n)
+        at += n
+    layout = api.KvLayout(1, blocks, block, kv_heads, dim)
+    cache = api.KvCache8(ctx, layout, codes=codes, scales=scales)
+    cu = np.concatenate([[0], np.cumsum(news)])
+    pos = np.concatenate([np.arange(c - n, c) for c, n in zip(contexts, news)])
+    q = torch.tensor(rng.standard_normal((int(cu[-1]), heads, dim)), dtype=torch.float32, device="cuda")
+    plan = api.StepPlan(ctx, block, i32(tables), lens=i32(after), cu_rows=i32(cu), row_pos=i32(pos))
+    out = torch.full_like(q, 7.0)
+    api.PagedAttention8(layout, heads).run_device(q, out, cache, plan, max_seq_rows=max(news), max_context=max(contexts))
+    values, sc, want = codes.float().cpu().numpy()[0], scales.cpu().numpy()[0], np.zeros(q.shape)
+    for b in range(B):
+        r = slice(cu[b], cu[b + 1])
+        want[r] = weighted_reference(q[r].cpu().numpy(), values, sc, tables[b], pos[r], block, kind)[0]
+    error = np.linalg.norm(out.cpu().numpy() - want) / np.linalg.norm(want)
+    assert error <= 2.0 ** -20.5, error
