@@ -507,10 +507,11 @@ pi_status pi_model_read_layer(pi_ctx* ctx, const pi_model* model, int layer, int
 /* ---- the device side of a serving step over an 8-bit KV cache --------------------------------------------------
  * A step of a ragged batch without a round trip to the host: its block tables and slots are made on the device from the
  * lengths of its requests, its keys and values are stored as 8-bit codes, attention reads those, and its tokens are drawn
- * from logits on the device.  All pointers are device memory on the context's device, all calls are ordered on the
- * context's stream, allocate nothing, wait for nothing on the host and may be captured into a CUDA graph (after a first
- * call of the same kind outside one), which then needs the context, the pool and the tensors for as long as it is replayed;
- * none of them keeps scratch memory, so contexts and graphs never share any.
+ * from logits on the device.  pi_step_plan, pi_kv8_write, pi_kv8_attention, pi_sample and pi_kv8_copy_block take device
+ * memory on the context's device, are ordered on the context's stream, allocate nothing, wait for nothing on the host and
+ * may be captured into a CUDA graph (after a first call of the same kind outside one), which then needs the context, the
+ * pool and the tensors for as long as it is replayed; none of them keeps scratch memory, so contexts and graphs never
+ * share any.  (pi_kv8_pool_create may allocate; pi_kv8_read_token copies to the host and waits.)
  * No counterpart in the reference. */
 
 /* The arrays of a step, all the caller's.  Rows are numbered through, sequence by sequence. */
@@ -535,7 +536,7 @@ typedef struct {
  * table behind its length and tables behind the last sequence stay as they are.  The call changes none of its inputs:
  * the caller drops the first counts[1] ids from the free list.  Where the list runs out, or a row of the tables is full,
  * entries become -1 (or do not exist), slots become -1 and counts[2] says how many blocks were missing; rows beyond
- * max_rows are left out (counts[0] still counts them).  At most 16384 sequences; positions stay below 2^31. */
+ * max_rows are left out (counts[0] still counts them).  1 to 16384 sequences; positions stay below 2^31. */
 pi_status pi_step_plan(pi_ctx* ctx, const pi_step_arrays* arrays, const int32_t* start_dev, const int32_t* n_tokens_dev, int n_seqs,
                        const int32_t* free_dev, int n_free);
 

@@ -24,7 +24,8 @@ inline int pi_kv8_pitch_of(int head_dim) {
   return 0;
 }
 
-// Division of 0 <= n < 2^31 by a constant: a product and a shift.
+// Division of 0 <= n < 2^31 by a constant: a product and a shift (Granlund and Montgomery, "Division by invariant integers using
+// multiplication").
 struct pi_divisor {
   uint32_t mul = 0, shift = 0;
   pi_divisor() = default;

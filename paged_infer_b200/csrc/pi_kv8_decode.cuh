@@ -28,7 +28,7 @@
 // memory, then through the cluster's: no scratch in device memory, and the order of the sums is fixed.
 //
 // Measured: 16 sequences of 3000 to 4096, 32 query heads of 128 over 8, bf16, e4m3: 30 us, 3.9 TB/s; 64 of 256 to 2048, 32 over 4 of 64, f32,
-// int8: 22 us, 1.75 TB/s; one of 131072, 64 over 8 of 128: 104 us, 2.6 TB/s.  Bound: the latency of a warp's chain with sixteen warps an
+// int8: 22.6 us, 1.7 TB/s; one of 131072, 64 over 8 of 128: 108 us, 2.5 TB/s.  Bound: the latency of a warp's chain with sixteen warps an
 // SM, and for few long sequences the 16 CTAs of a cluster.
 #pragma once
 

@@ -26,9 +26,11 @@
 // both products of a head of 128 channels; around them come a multiplication, a maximum, an addition and half a conversion each, and
 // reading back the tile's output.
 //
-// Measured: 512 rows behind 3584 positions, 32 query heads of 128 over 8, bf16: 121 us, 266 TFLOP/s; 16 sequences of 1 to 256 rows in a
-// window of 1024, 32 over 4 of 64, f32 (two planes): 178 us.  Leaving out the exponentials, the widening, the products or the output's
-// way back saves at most 8 % each: the chain of one tile of rows is what takes the time, and tensor memory has no room for a second.
+// Measured: 512 rows behind 3584 positions, 32 query heads of 128 over 8, bf16: 108 us, 298 TFLOP/s; 16 sequences of 1 to 256 rows in a
+// window of 1024, 32 over 4 of 64, f32 (two planes): 165 us.  Leaving out the exponentials, the widening, the products or the output's
+// way back saved at most 8 % each (of 121 us, with slower waits): the chain of one tile of rows is what takes the time.  Tensor memory has no room
+// for a second one in this layout (two buffers of scores, P, the tile's output and Q beside each other).  Heads of 128 keep 64 outputs and 64
+// scores in a row thread's 152 registers, which spills some 150 bytes a thread (one plane; 50 with two, none at 64).
 #include <math.h>
 
 #include <algorithm>

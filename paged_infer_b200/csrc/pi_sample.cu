@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   goal = min(goal, total - 1);
   // the first token whose running sum exceeds the goal: its CTA finds the warp whose run holds it, deals that run to all warps, and the
   // warp whose part holds it scans that.  (64 rows of 128256 without top-k or top-p:
-  // 49 us, 60 where that warp scans its whole run.)
+  // 42 us, 60 where that warp scans its whole run.)
   if (goal >= ahead && goal < ahead + held_here) {
     unsigned long long before = ahead, taken = used_here;
     for (bool dealt = false;; dealt = true) {
