@@ -14,15 +14,16 @@ namespace {
 thread_local std::string g_create_error;
 
 // What contexts of one device share: its properties, asked for once, and their error records, cut from one allocation, so that a
-// context on a stream of the caller's is created without a call to the device and destroyed without cudaFree, which waits for all of
-// the device's streams.  (On a stream of the caller's: 2 us to create and 7 to destroy; with cudaGetDeviceProperties and an allocation each 890, and whatever the device was busy with.)
+// context on a stream of the caller's, beside another one, is created without a call to the device and destroyed without cudaFree,
+// which waits for all of the device's streams: 2 us to create and 7 to destroy (890 with cudaGetDeviceProperties and an allocation each,
+// and then whatever the device was busy with).
 constexpr int kDevices = 64, kErrRecords = 256;
 struct DeviceShare {
   bool known = false;
   int major = 0, minor = 0, sm_count = 0, smem_optin = 0;
   int* records = nullptr;             // kErrRecords of PI_DEV_ERR_WORDS, all zero but those in use
   unsigned char next[kErrRecords];    // records that are free
-  int free = 0;
+  int free = 0, users = 0;            // contexts with one of them; the last one frees the allocation
 };
 std::mutex g_share_mutex;
 DeviceShare g_share[kDevices];
@@ -59,6 +60,7 @@ cudaError_t take_record(DeviceShare& d, int** out, bool* owned) {
   *owned = d.free == 0;
   if (*owned) return zeros(out, bytes);
   *out = d.records + (size_t)d.next[--d.free] * PI_DEV_ERR_WORDS;
+  ++d.users;
   return cudaSuccess;
 }
 }  // namespace
@@ -235,10 +237,14 @@ void pi_ctx_destroy(pi_ctx* ctx) {
   for (cudaEvent_t e : ctx->prof_events) cudaEventDestroy(e);
   if (ctx->own_dev_err) {
     cudaFree(ctx->dev_err);
-  } else if (clean) {
+  } else {
     std::lock_guard<std::mutex> lock(g_share_mutex);
     DeviceShare& share = g_share[ctx->device];
-    share.next[share.free++] = (unsigned char)((ctx->dev_err - share.records) / PI_DEV_ERR_WORDS);
+    if (clean) share.next[share.free++] = (unsigned char)((ctx->dev_err - share.records) / PI_DEV_ERR_WORDS);
+    if (--share.users == 0) {
+      cudaFree(share.records);
+      share.records = nullptr;
+    }
   }
   if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
   delete ctx;
