@@ -19,8 +19,7 @@
 // Warp 16: issues the products (17-19 are there because registers are dealt to four warps at a time); the scores of tile j + 1 run
 // while the rows work on tile j.
 // Hand-offs go through mbarriers; every wait is bounded and raises the context's error word instead of hanging, and the tile's rows
-// become NaN.  Where there are few
-// tiles of rows, a cluster shares the positions of one and joins its CTAs' outputs through shared memory.
+// become NaN.  Where there are few tiles of rows, a cluster shares the positions of one and joins its CTAs' outputs through shared memory.
 //
 // Bound: the rows' threads.  A tile of 128 by 128 needs 16384 exponentials, of which an SM makes 16 a clock: 1024 clocks, as long as
 // both products of a head of 128 channels; around them come a multiplication, a maximum, an addition and half a conversion each, and
