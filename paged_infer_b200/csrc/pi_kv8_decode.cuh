@@ -5,8 +5,9 @@
 // holds exactly, so both products run on the tensor cores (m16n8k16, f32 accumulators) with the CACHE as the wide operand:
 //     S^T[16 tokens][8 columns] = K q^T,    O^T[dims][8 columns] += scale_v (V^T P^T),    a column = one query head of one row.
 // A group of eight query heads fills a product; four need no more of them than eight would.  f32 queries, and the weights of f32
-// outputs, are two f16 planes (22 bits); those of bf16 and f16 outputs are one.  Queries are brought to [-1, 1] by a power of two
-// per column, weights to 2^15 at most, so that neither leaves f16's normal range; the scales stay in f32.
+// outputs, are two f16 planes (22 bits); those of bf16 and f16 outputs are one.  Queries are brought to between 2^14 and 2^15 by a power
+// of two per column, so that channels 2^29 below its largest are normal numbers of f16 still (2^17 with both planes' bits), weights to
+// 2^15 at most; the scales stay in f32.
 //
 // Codes go from memory straight to the registers that feed the products: the k index of a product may be permuted at will, so a
 // lane takes whole words of a token's codes for K, and, for V, of the four tokens whose weights it holds; pairs of tokens are put
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
     look();
 
     // the first codes are under way; meanwhile the columns' queries become b fragments: eight lanes a column, four channels at a time,
-    // each column times the power of two that brings it to [-1, 1]
+    // each column times the power of two that brings its largest to 2^14 or more
     for (int c = tid >> 3; c < COLS; c += warps * 4) {
       const int l8 = lane & 7, rel = col0 + c < ncols ? p.by_group(col0 + c) : 0, row = row_begin + rel;
       const bool live = col0 + c < ncols;
@@ -244,8 +245,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       // 2^(e - 127) <= most < 2^(e - 126); both powers below stay normal
-      const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);
-      const float shrink = __uint_as_float((253u - e) << 23);   // 2^(126 - e)
+      const uint32_t e = min(max(__float_as_uint(most) >> 23, 17u), 252u);
+      const float shrink = __uint_as_float((268u - e) << 23);   // 2^(141 - e)
 #pragma unroll
       for (int i = 0; i < PITCH / 32; ++i) {
         const int d = 4 * (l8 + 8 * i), piece = d / (G::KB * 4), in = d % (G::KB * 4), to = (piece * (G::KB / 4) + in % G::KB / 4) * PLANES;
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
         const int pos = live ? p.row_pos[row] : -1;
         s_lo[c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         s_hi[c] = pos;
-        s_factor[c] = __uint_as_float((e + 1) << 23) * p.scale2;   // 2^(e - 126)
+        s_factor[c] = __uint_as_float((e - 14) << 23) * p.scale2;   // 2^(e - 141)
       }
     }
     __syncthreads();

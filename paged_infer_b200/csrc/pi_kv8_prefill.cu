@@ -3,7 +3,7 @@
 //
 // A CTA owns 128 (row, query head) pairs of one sequence and KV head, one per TMEM lane, and walks the positions that they see in tiles
 // of 128 columns (64 for heads of 128 with two planes): eight times 16 tokens, each of one block and with one pair of scales.  Codes are
-// widened to f16, which holds them exactly; queries (brought to [-1, 1] by a power of two per row) and weights are f16 too, in two planes (22 bits) for f32 tensors:
+// widened to f16, which holds them exactly; queries (brought to 2^14 to 2^15 by a power of two per row) and weights are f16 too, in two planes (22 bits) for f32 tensors:
 //     scores  S = Q K^T        A = Q (written once),  B = codes of K, [token][channel]
 //     output  O = P V          A = P,                 B = codes of V transposed, [channel][token]
 // A row's thread multiplies the K scale in as it reads its scores, and weighs exp(score) by V scale / r, r a power of two above the
@@ -247,9 +247,9 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 #pragma unroll
       for (int b = 0; b < 4; ++b) most = fmaxf(most, fabsf(x[b]));
     }
-    const uint32_t e = min(max(__float_as_uint(most) >> 23, 2u), 252u);   // both powers stay normal
-    const float shrink = __uint_as_float((253u - e) << 23);
-    factor = __uint_as_float((e + 1) << 23) * p.scale2;
+    const uint32_t e = min(max(__float_as_uint(most) >> 23, 17u), 252u);   // both powers stay normal
+    const float shrink = __uint_as_float((268u - e) << 23);
+    factor = __uint_as_float((e - 14) << 23) * p.scale2;
 #pragma unroll 2
     for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 16) {
       uint32_t hi[8], lo[8];

@@ -246,3 +246,33 @@ def test_f32_rows_against_64_bits_as_a_whole(ctx, kind, heads, kv_heads, dim, co
         want[r] = weighted_reference(q[r].cpu().numpy(), values, sc, tables[b], pos[r], block, kind)[0]
     error = np.linalg.norm(out.cpu().numpy() - want) / np.linalg.norm(want)
     assert error <= 2.0 ** -20.5, error
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim,news", [(64, 1), (128, 2), (96, 1), (64, 60), (128, 60)])
+def test_an_outlier_channel_of_the_query(ctx, kind, dtype, dim, news):
+    """A query channel 2^20 times the others, where the keys are zero: scores are made of the others alone and keep their precision."""
+    rng = np.random.default_rng(dim + news)
+    block, heads, kv_heads, context = 16, 8, 2, 90
+    blocks = -(-context // block)
+    shape = (1, blocks, kv_heads, 2, block, pitch_of(dim))
+    values = np.clip(np.round(rng.standard_normal(shape) * 35), -120, 120).astype(np.float32)
+    if kind == "e4m3":
+        values = torch.tensor(values).to(torch.float8_e4m3fn).float().numpy()
+    values[..., dim:] = 0
+    values[..., 0, :, 5] = 0
+    q = rng.uniform(0.5, 1.0, (news, heads, dim)) * rng.choice([-1, 1], (news, heads, dim)) * 2.0 ** -5
+    q[..., 5] = 2.0 ** 15
+    q = torch.tensor(q, device="cuda").to(TYPES[dtype])
+    scales = np.full(shape[:4], 1 / 40, np.float32)
+    scales[..., 0] = 2.0 ** 5 / 30                       # scores of a few units
+    table, pos = rng.permutation(blocks), np.arange(context - news, context)
+    layout = api.KvLayout(1, blocks, block, kv_heads, dim)
+    cache = api.KvCache8(ctx, layout, codes=torch.tensor(values, device="cuda").to(TORCH[kind]), scales=torch.tensor(scales, device="cuda"))
+    plan = api.StepPlan(ctx, block, i32(table[None]), lens=i32([blocks]), cu_rows=i32([0, news]), row_pos=i32(pos))
+    out = torch.full_like(q, 7.0)
+    api.PagedAttention8(layout, heads).run_device(q, out, cache, plan)
+    want, weighed, mass = weighted_reference(q.float().cpu().numpy(), values[0], scales[0], table, pos, block, kind)
+    off = np.abs(out.float().cpu().numpy() - want) - attention_tolerance(want, weighed, mass, dim, dtype)
+    assert not (off > 0).any(), (off.max(), (off > 0).sum())
