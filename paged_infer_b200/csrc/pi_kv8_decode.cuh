@@ -14,11 +14,10 @@
 // together by byte permutes.  The next tile's K codes are requested as soon as this tile's are used up, its V codes likewise, so that
 // every warp has loads under way all the time without a second set of registers and without shared memory.
 //
-// int8 codes become f16 by a byte permute into the mantissa of 1024 (1024 + 128 + code), and 1152 is subtracted from every pair.  Only
-// V's, with one plane, keep it, and the accumulators start from -1152 times the sum of the weights instead: a result is off by up to
-// 1152 x 2^-23 of its V scale for that, 2^-13 of a step of the codes.  Not K's: a score would be off by as much for every unit of the query,
-// which is a lot beside a channel of large codes in which the query is small, where the other codes are few steps (a tenth of a weight
-// at 256 channels).  (One context of 131072: 108 us, 104 with K's left in; 16 of 3000 to 4096, int8: 32.1 and 31.4.)
+// int8 codes become f16 by a byte permute into the mantissa of 1024 (1024 + 128 + code), and 1152 is subtracted from every pair.  (Left in, with
+// accumulators that start from -1152 times the sum of the other operand, it costs scores their precision beside a channel of large codes
+// in which the query is small, and results theirs beside a token of nearly all the weight and small values; it takes longer, too: one
+// context of 131072 108 us instead of 106.)
 //
 // Products add to their accumulators with truncation, up to an ulp of the sum each.  So the two planes of a query have accumulators of their
 // own (terms of a code and 11 bits leave little to truncate, those of the second plane are small), and the first plane's sums are
@@ -48,11 +47,11 @@ __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16_from(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {   // d = a b + c, c the same for all rows
+__device__ __forceinline__ void mma_f16_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // d = a b
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // of an 8 x 8 tile of 16-bit values, a row per four lanes
   uint32_t y;
@@ -72,7 +71,6 @@ __device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* from) {
     to[0] = __ldcs(reinterpret_cast<const uint32_t*>(from));
   }
 }
-constexpr float kBias = 1152.f;
 
 template <int PITCH>
 struct Geometry {
@@ -105,7 +103,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
   using S = Shape<PITCH, NT>;
   constexpr int COLS = S::cols, TT = S::TT, LINE = S::line;
   constexpr int RUN = PLANES == 2 ? 8 : G::ksteps;   // steps of 16 channels
-  constexpr bool BIASED = KIND == PI_INT8 && PLANES == 1;
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
   unsigned char* s_queries = smem;
@@ -318,10 +315,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
 #pragma unroll
         for (int e = 0; e < TT; ++e) {
           const uint32_t w0 = unsign<KIND>(kw[e][0][j]), w1 = unsign<KIND>(kw[e][1][j]);
-          a[e][0] = widen<KIND, false>(w0, false);
-          a[e][1] = widen<KIND, false>(w1, false);
-          a[e][2] = widen<KIND, false>(w0, true);
-          a[e][3] = widen<KIND, false>(w1, true);
+          a[e][0] = widen<KIND>(w0, false);
+          a[e][1] = widen<KIND>(w1, false);
+          a[e][2] = widen<KIND>(w0, true);
+          a[e][3] = widen<KIND>(w1, true);
         }
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl)
@@ -331,7 +328,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
 #pragma unroll
             for (int e = 0; e < TT; ++e) {
               float* to = pl == 1 ? low[e][n] : j < RUN ? s[e][n] : run[e][n];
-              if (pl == 1 ? j == 0 : j % RUN == 0) mma_f16_from(to, a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y, 0.f, 0.f);
+              if (pl == 1 ? j == 0 : j % RUN == 0) mma_f16_new(to, a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y);
               else mma_f16(to, a[e][0], a[e][1], a[e][2], a[e][3], b.x, b.y);
               if (pl == 0 && j >= RUN && (j % RUN == RUN - 1 || j == G::ksteps - 1)) {
 #pragma unroll
@@ -422,21 +419,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
 #pragma unroll
       for (int e = 0; e < TT; ++e) {
         // the V scale per column; one that is not finite reaches the columns that see the tile and no others
-        float unit[NT][2], p_bias[NT][2];
+        float unit[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c)
             unit[n][c] = all || (token[e] + valid[e] > lo[n][c] && token[e] <= hi[n][c] && valid[e] > 0) ? scale[e].y : 0.f;
-            p_bias[n][c] = 0.f;
-          }
-          if constexpr (BIASED) {   // the sum of the weights as they were rounded: a product with ones
-            float d[4];
-            constexpr uint32_t ones = 0x3c003c00u;
-            mma_f16_from(d, ones, ones, ones, ones, pw[e][n][0][0], pw[e][n][1][0], 0.f, 0.f);
-            p_bias[n][0] = -kBias * d[0];
-            p_bias[n][1] = -kBias * d[1];
-          }
         }
 #pragma unroll
         for (int w = 0; w < PITCH / 32; ++w) {
@@ -444,11 +432,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<PITCH, NT>::min_ctas) kv
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t x = __byte_perm(v0, v1, half ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, half ? 0x7362 : 0x5140);
-            const uint32_t a0 = widen<KIND, BIASED>(x, false), a1 = widen<KIND, BIASED>(x, true), a2 = widen<KIND, BIASED>(y, false), a3 = widen<KIND, BIASED>(y, true);
+            const uint32_t a0 = widen<KIND>(x, false), a1 = widen<KIND>(x, true), a2 = widen<KIND>(y, false), a3 = widen<KIND>(y, true);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float d[4];
-              mma_f16_from(d, a0, a1, a2, a3, pw[e][n][0][0], pw[e][n][1][0], p_bias[n][0], p_bias[n][1]);
+              mma_f16_new(d, a0, a1, a2, a3, pw[e][n][0][0], pw[e][n][1][0]);
               if constexpr (PLANES == 2) mma_f16(d, a0, a1, a2, a3, pw[e][n][0][1], pw[e][n][1][1]);
               float* o = out[n][2 * w + half];
 #pragma unroll

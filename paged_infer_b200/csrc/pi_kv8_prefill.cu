@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
         for (int c = 0; c < CHUNKS; ++c) {
           const uint32_t a = unsign<KIND>(cur.k[2 * c]), b = unsign<KIND>(cur.k[2 * c + 1]);
           const int chunk = HD == 128 ? c : k_half * CHUNKS + c, sub = HD == 128 ? k_half : 0;
-          st_shared((kdst ^ chunk << 4) + sub * (TILE * 128), widen<KIND, false>(a, false), widen<KIND, false>(a, true), widen<KIND, false>(b, false), widen<KIND, false>(b, true));
+          st_shared((kdst ^ chunk << 4) + sub * (TILE * 128), widen<KIND>(a, false), widen<KIND>(a, true), widen<KIND>(b, false), widen<KIND>(b, true));
         }
       }
       {   // V: eight tokens of a channel are 16 bytes, [part][channel][128 bytes] swizzled
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) kv8_prefill_kernel(const Prefill
 #pragma unroll
             for (int one = 0; one < 2; ++one) {
               const int i = w * 4 + half * 2 + one;   // of this thread's channels, which begin at a multiple of their number
-              st_shared((vdst ^ i << 4) + i * 128, widen<KIND, false>(x[0], one), widen<KIND, false>(x[1], one), widen<KIND, false>(x[2], one), widen<KIND, false>(x[3], one));
+              st_shared((vdst ^ i << 4) + i * 128, widen<KIND>(x[0], one), widen<KIND>(x[1], one), widen<KIND>(x[2], one), widen<KIND>(x[3], one));
             }
           }
         }

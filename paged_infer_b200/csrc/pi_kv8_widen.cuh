@@ -15,13 +15,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two codes as f16: bytes 0 and 1, or 2 and 3, of a word.  int8 (its sign bit flipped): 1024 + (code + 128) in the mantissa, less 1152
-// unless that stays in.
-template <int KIND, bool BIASED>
+// Two codes as f16: bytes 0 and 1, or 2 and 3, of a word.  int8 (its sign bit flipped): 1024 + (code + 128) in the mantissa, less 1152.
+template <int KIND>
 __device__ __forceinline__ uint32_t widen(uint32_t w, bool high) {
   if (KIND == PI_INT8) {
     const uint32_t h = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
-    if (BIASED) return h;
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&v);
   }

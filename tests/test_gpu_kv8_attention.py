@@ -276,3 +276,36 @@ def test_an_outlier_channel_of_the_query(ctx, kind, dtype, dim, news):
     want, weighed, mass = weighted_reference(q.float().cpu().numpy(), values[0], scales[0], table, pos, block, kind)
     off = np.abs(out.float().cpu().numpy() - want) - attention_tolerance(want, weighed, mass, dim, dtype)
     assert not (off > 0).any(), (off.max(), (off > 0).sum())
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype,nats", [("f32", 10), ("bf16", 10), ("f16", 10)])
+@pytest.mark.parametrize("dim,news,context", [(64, 1, 65), (128, 2, 80), (96, 1, 70), (64, 60, 120), (128, 60, 120)])
+def test_a_token_of_nearly_all_the_weight_and_no_value(ctx, kind, dtype, nats, dim, news, context):
+    """A first token `nats` above the others whose values are zero: results are made of the others, whose weights keep their precision.  One
+    channel makes the scores, whose sums are exact."""
+    rng = np.random.default_rng(dim + news)
+    block, heads, kv_heads = 16, 4, 2
+    blocks = -(-context // block)
+    values = np.zeros((1, blocks, kv_heads, 2, block, pitch_of(dim)), np.float32)
+    values[..., 1, :, :dim] = np.clip(np.round(rng.standard_normal(values[..., 1, :, :dim].shape) * 35), -120, 120)
+    values[..., 0, :, 0] = rng.integers(-7, 8, values[..., 0, :, 0].shape)
+    values[0, 0, :, 0, 0, 0], values[0, 0, :, 1, 0] = 120, 0
+    if kind == "e4m3":
+        values = torch.tensor(values).to(torch.float8_e4m3fn).float().numpy()
+    scales = np.full(values.shape[:4], 1 / 40, np.float32)
+    scales[..., 0] = nats / 120 * dim ** 0.5
+    q = np.zeros((news, heads, dim), np.float32)
+    q[..., 0] = 1.0
+    q = torch.tensor(q, device="cuda").to(TYPES[dtype])
+    table = np.arange(blocks)
+    pos = np.arange(context - news, context)
+    layout = api.KvLayout(1, blocks, block, kv_heads, dim)
+    cache = api.KvCache8(ctx, layout, codes=torch.tensor(values, device="cuda").to(TORCH[kind]), scales=torch.tensor(scales, device="cuda"))
+    plan = api.StepPlan(ctx, block, i32(table[None]), lens=i32([blocks]), cu_rows=i32([0, news]), row_pos=i32(pos))
+    out = torch.full_like(q, 7.0)
+    api.PagedAttention8(layout, heads).run_device(q, out, cache, plan)
+    want, weighed, mass = weighted_reference(q.float().cpu().numpy(), values[0], scales[0], table, pos, block, kind)
+    tolerance = attention_tolerance(want, weighed, mass, 2, dtype) + (2.0 ** -25 if dtype == "f16" else 0)   # half of f16's smallest step
+    off = np.abs(out.float().cpu().numpy() - want) - tolerance
+    assert not (off > 0).any(), (off.max(), (off > 0).sum())
