@@ -9,8 +9,8 @@
 // A row's thread multiplies the K scale in as it reads its scores, and weighs exp(score) by V scale / r, r a power of two above the
 // largest product of weight and V scale in the tile, so that P stays in f16's range whatever the scales are, and what a large scale
 // takes from a small one's bits it takes by what it adds to the result; the product of a tile is read
-// back, multiplied by r and added to the row's f32 output in registers.  The running maximum may lag 2^8 behind, so that the output
-// is hardly ever rescaled.
+// back, multiplied by r and added to the row's f32 output in registers.  The running maximum may lag 2^3 behind, so that the output
+// is seldom rescaled.
 //
 // Warps 0-7: two threads per row, each with half of a tile's columns and half of the output's channels; they share the row's running
 // maximum through shared memory, once a tile (one thread per row leaves every scheduler one such warp: 151 us where two take 143).

@@ -279,7 +279,7 @@ def test_an_outlier_channel_of_the_query(ctx, kind, dtype, dim, news):
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
-@pytest.mark.parametrize("dtype,nats", [("f32", 10), ("bf16", 10), ("f16", 10)])
+@pytest.mark.parametrize("dtype,nats", [("f32", 10), ("bf16", 10), ("f16", 10), ("f32", 17), ("bf16", 20), ("f16", 20)])
 @pytest.mark.parametrize("dim,news,context", [(64, 1, 65), (128, 2, 80), (96, 1, 70), (64, 60, 120), (128, 60, 120)])
 def test_a_token_of_nearly_all_the_weight_and_no_value(ctx, kind, dtype, nats, dim, news, context):
     """A first token `nats` above the others whose values are zero: results are made of the others, whose weights keep their precision.  One
