@@ -21,14 +21,14 @@
 //
 // Products add to their accumulators with truncation, up to an ulp of the sum each.  So the two planes of a query have accumulators of their
 // own (terms of a code and 11 bits leave little to truncate, those of the second plane are small), and the first plane's sums are
-// taken over 128 channels and added with rounding.  (f32 results against 64 bits in random calls: 0.8 times the error of f32 sums in torch in
-// the median, 5.3e-7 of the result at most; with one accumulator 1.4 times and 1.2e-6.  64 sequences of heads of 64: 22.6 us, 22.3 with one.)
+// taken over 128 channels and added with rounding.  (f32 results against 64 bits in random calls: 0.9 times the error of f32 sums in torch in
+// the median, 5.6e-7 of the result at most; with one accumulator 1.4 times and 1.2e-6.  64 sequences of heads of 64: 22.6 us, 22.3 with one.)
 //
 // The tokens of a sequence are dealt to the warps of a CTA and to the CTAs of a cluster; partial results are joined through shared
 // memory, then through the cluster's: no scratch in device memory, and the order of the sums is fixed.
 //
 // Measured: 16 sequences of 3000 to 4096, 32 query heads of 128 over 8, bf16, e4m3: 30 us, 3.9 TB/s; 64 of 256 to 2048, 32 over 4 of 64, f32,
-// int8: 22.6 us, 1.7 TB/s; one of 131072, 64 over 8 of 128: 108 us, 2.5 TB/s.  Bound: the latency of a warp's chain with sixteen warps an
+// int8: 22.6 us, 1.7 TB/s; one of 131072, 64 over 8 of 128: 106 us, 2.5 TB/s.  Bound: the latency of a warp's chain with sixteen warps an
 // SM, and for few long sequences the 16 CTAs of a cluster.
 #pragma once
 
