@@ -57,7 +57,7 @@ class Context:
         self.device, self.rank, self.tp = device, rank, tp
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:   # module globals are gone at interpreter exit
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_ctx_destroy(self.handle)
             self.handle = None
 
@@ -228,7 +228,7 @@ class Projection:
         return cls.f32(ctx, np.asarray(bf16_bits, np.uint16))
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:   # module globals are gone at interpreter exit
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_linear_destroy(self.handle)
             self.handle = None
 
@@ -408,7 +408,7 @@ class KvCache:
         self.handle = h
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:   # module globals are gone at interpreter exit
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_kv_pool_destroy(self.handle)
             self.handle = None
 
@@ -606,7 +606,7 @@ class KvCache8:
         self.handle = h
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:   # module globals are gone at interpreter exit
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_kv8_pool_destroy(self.handle)
             self.handle = None
 
@@ -705,7 +705,7 @@ class StatePool:
         self.handle = h
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_state_pool_destroy(self.handle)
             self.handle = None
 
@@ -830,7 +830,7 @@ class LayeredModel(_Steps):
         return self
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_model_destroy(self.handle)
             self.handle = None
 
@@ -924,7 +924,7 @@ class LlamaWeights(_Steps):
         return self
 
     def close(self):
-        if getattr(self, "handle", None) and _lib is not None:   # module globals are gone at interpreter exit
+        if getattr(self, "handle", None) and _lib is not None and _lib.lib is not None:   # globals, here and there, are gone at interpreter exit
             _lib.lib().pi_model_destroy(self.handle)
             self.handle = None
 
